@@ -306,6 +306,144 @@ int mamw_ns_direct(int op, const uint16_t* X, const uint16_t* S, uint16_t* out,
                    void* workspace, size_t workspace_bytes,
                    mamw_stream_t stream);
 
+/* ==== Objectives: losses over rows of logits and their gradients ============ *
+ * The part of a training step before the optimizer: log-probabilities of tokens,
+ * a clipped policy loss, a preference loss over pairs of sequences and
+ * distillation from a teacher's top logits, each with d loss / d logits.  No
+ * counterpart in the reference, which starts at gradients.
+ *
+ * A row holds the logits x of one token.  With T the temperature,
+ *     M = max x,  s = sum_j exp((x_j - M)/T),  q_j = exp((x_j - M)/T) / s,
+ *     log q_j = (x_j - M)/T - log s;
+ * everything between the logits and the gradient is fp32.  Rows that do not count
+ * (token == ignore_index, mask false) are not read: they give 0 and gradients
+ * of 0.  A token or teacher index beyond the vocabulary reads nothing and gives
+ * NaN.  Rows are numbered outer * inner_count + inner; outputs, one value a row,
+ * and gradients (rows x vocab, the logits' type) are dense.                   */
+#define MAMW_F32  0
+#define MAMW_BF16 1
+#define MAMW_F16  2
+#define MAMW_I32  3
+#define MAMW_I64  4
+#define MAMW_BOOL 5 /* one byte: 0 or 1 */
+
+/* outer x inner rows of `vocab` consecutive elements; strides in elements.    */
+typedef struct mamw_rows {
+    const void* data;
+    int64_t     outer, inner;  /* >= 0, their product below 2^31 */
+    int64_t     vocab;         /* 1 .. 2^31 - 1                   */
+    int64_t     outer_stride, inner_stride;
+    int32_t     type;          /* MAMW_F32, MAMW_BF16 or MAMW_F16 */
+    int32_t     reserved;      /* must be 0                       */
+} mamw_rows;
+
+/* One value (or `k` consecutive ones) for each of those rows; a stride may be 0. */
+typedef struct mamw_per_row {
+    const void* data;
+    int64_t     outer_stride, inner_stride;
+    int32_t     type;
+    int32_t     reserved;      /* must be 0 */
+} mamw_per_row;
+
+/* logprobs[r] = log q_token; entropy[r] = -sum_j q_j log q_j (entropy may be NULL);
+ * stats[2r], stats[2r+1] = M, s of the rows that count, for mamw_logits_grad (may be NULL). */
+int mamw_token_logprobs(const mamw_rows* logits, const mamw_per_row* tokens,
+                        int64_t ignore_index, float temperature,
+                        float* logprobs, float* entropy, float* stats,
+                        mamw_stream_t stream);
+
+/* grad_j = (a [j = token] - q_j (a + h (log q_j + entropy))) / T with
+ * a = scale * coef[r], h = scale * entropy_coef[r] (no such term where
+ * entropy_coef is NULL) and *scale on the device (NULL: 1).                   */
+int mamw_logits_grad(const mamw_rows* logits, const mamw_per_row* tokens,
+                     int64_t ignore_index, float temperature,
+                     const float* stats, const mamw_per_row* coef,
+                     const mamw_per_row* entropy_coef, const float* entropy,
+                     const float* scale, void* grad, mamw_stream_t stream);
+
+/* Clipped policy loss.  With l = log q_token, r = exp(l - old), A the advantage
+ * and d = ref - l, a row's loss is
+ *     -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)
+ * and the result the sum of scale * w * (row's loss): w = 1 / (rows that count), or
+ * with by_sequence 1 / (those of its sequence * sequences that have any).
+ * Sequences: `offsets` (sequences + 1 places among the rows, not falling; a
+ * row in none of them does not count with by_sequence), or one for each outer
+ * index where it is NULL.
+ * result[0..2] = loss, sum of w (exp(d) - d - 1), sum of w over the rows whose
+ * gradient the clamp removes.  grad may be NULL.                              */
+typedef struct mamw_policy {
+    mamw_per_row   tokens;       /* MAMW_I32, MAMW_I64               */
+    mamw_per_row   old_logprobs; /* MAMW_F32                         */
+    mamw_per_row   advantages;   /* MAMW_F32                         */
+    mamw_per_row   ref_logprobs; /* MAMW_F32; data NULL: no KL term  */
+    const int64_t* offsets;      /* device; NULL: outer indices      */
+    int64_t        sequences;
+    int64_t        ignore_index;
+    float          clip_low, clip_high, kl_coef, temperature, scale;
+    int32_t        by_sequence;
+} mamw_policy;
+
+int mamw_policy_workspace_bytes(const mamw_rows* logits, const mamw_policy* p, size_t* bytes);
+int mamw_policy_loss(const mamw_rows* logits, const mamw_policy* p, float* result, float* logprobs,
+                     void* grad, void* workspace, size_t workspace_bytes, mamw_stream_t stream);
+/* The gradient again, times *scale; nothing where *scale is 1 and unless_one is
+ * set.  The workspace is that of the loss, as it was left.                    */
+int mamw_policy_grad(const mamw_rows* logits, const mamw_policy* p, const float* scale, int unless_one,
+                     void* grad, void* workspace, size_t workspace_bytes, mamw_stream_t stream);
+
+/* Preference loss over pairs of sequences, i < pairs = sequences / 2 against
+ * i + pairs.  With L_s the sum of log q_token over the rows of sequence s that count
+ * (their mean with length_average; 0 where there are none),
+ *     rewards_s = beta (L_s - ref_s),  h = rewards_i - rewards_{i+pairs},
+ *     MAMW_SIGMOID: -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h)
+ *     MAMW_IPO:     (h / beta - 1 / (2 beta))^2
+ *     MAMW_HINGE:   max(0, 1 - h),
+ * result[0] = the mean over the pairs.  logprobs = L_s, rewards: one value a sequence.
+ * stats (2 a row) and coef (1 a row) are for mamw_logits_grad.                */
+#define MAMW_SIGMOID 0
+#define MAMW_IPO     1
+#define MAMW_HINGE   2
+typedef struct mamw_preference {
+    mamw_per_row   tokens;
+    const float*   ref_logprobs; /* one a sequence; NULL: 0s */
+    const int64_t* offsets;      /* as for mamw_policy       */
+    int64_t        sequences;    /* even, at least 2         */
+    int64_t        ignore_index;
+    float          beta, smoothing, temperature;
+    int32_t        kind, length_average;
+    int32_t        reserved;     /* must be 0                */
+} mamw_preference;
+
+int mamw_preference_workspace_bytes(const mamw_rows* logits, const mamw_preference* p, size_t* bytes);
+int mamw_preference_loss(const mamw_rows* logits, const mamw_preference* p, float* result, float* logprobs,
+                         float* rewards, float* stats, float* coef, void* workspace,
+                         size_t workspace_bytes, mamw_stream_t stream);
+
+/* Distillation from the k first logits t of a teacher.  p = softmax(t / T) over
+ * the k, or with teacher_lse = log sum exp(t / T) over the teacher's whole
+ * vocabulary p = exp(t / T - lse), and then all other entries together are one more:
+ *     row = sum_k p_k (log p_k - log q_k)  [+ P log(P / Q)]
+ *     P = max(1 - sum_k p_k, 2^-20),  Q = sum of q_j over the other entries
+ * (P = 0 where there are no others), result[0] = scale T^2 times the mean over the rows
+ * that count.  Entries with a negative index or a logit of -inf are left out.
+ * k is at most MAMW_MAX_TEACHER; with teacher_lse vocab is at most 2^20.      */
+#define MAMW_MAX_TEACHER 1024
+typedef struct mamw_distill {
+    mamw_per_row teacher_logits;  /* k a row: MAMW_F32, MAMW_BF16, MAMW_F16 */
+    mamw_per_row teacher_indices; /* k a row: MAMW_I32, MAMW_I64            */
+    mamw_per_row teacher_lse;     /* MAMW_F32; data NULL: renormalised      */
+    mamw_per_row mask;            /* MAMW_BOOL; data NULL: all rows count   */
+    int64_t      k;
+    float        temperature, scale;
+} mamw_distill;
+
+int mamw_distill_workspace_bytes(const mamw_rows* logits, const mamw_distill* p, size_t* bytes);
+int mamw_distill_loss(const mamw_rows* logits, const mamw_distill* p, float* result, void* grad,
+                      void* workspace, size_t workspace_bytes, mamw_stream_t stream);
+/* As mamw_policy_grad. */
+int mamw_distill_grad(const mamw_rows* logits, const mamw_distill* p, const float* scale, int unless_one,
+                      void* grad, void* workspace, size_t workspace_bytes, mamw_stream_t stream);
+
 /* ==== Profiling (opt-in) ==================================================== *
  * Between mamw_prof_start() and mamw_prof_stop(), every kernel launched by the
  * library is timed with a pair of HIP events bound to its dispatch.

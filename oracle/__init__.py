@@ -13,6 +13,8 @@ bf16    round-to-nearest-even bfloat16 emulation on float32 arrays
 adamw   triton_adam.py:53-59 (update) and :132-153 (step loop semantics)
 muon    triton_muon.py:327-372 / torch/optim/_muon.py:31-84,285-318
         (momentum, Nesterov blend, Newton-Schulz, LR scale, update)
+objectives  token log-probabilities, policy, preference and distillation losses
+        (no counterpart in the reference), float64
 
 Every function is pinned by tests in ``tests/test_oracle_*.py`` against
 closed forms, invariants and the torch.optim library routines the reference
@@ -20,4 +22,4 @@ delegates to (``PyTorchMuonAdamW``, optimizer.py:178-260), and by the golden
 fixtures in ``tests/golden/``.
 """
 
-from . import adamw, bf16, muon  # noqa: F401
+from . import adamw, bf16, muon, objectives  # noqa: F401

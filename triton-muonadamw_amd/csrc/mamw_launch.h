@@ -35,6 +35,13 @@ enum KernelId : int32_t {
     K_DIRECT_UPDATE,
     K_DIRECT_APPLY,
     K_DIRECT_PACK,
+    K_OBJ_LOGPROBS,
+    K_OBJ_GRAD,
+    K_OBJ_COUNT,
+    K_OBJ_RESULT,
+    K_OBJ_POLICY,
+    K_OBJ_PAIRS,
+    K_OBJ_DISTILL,
     K_COUNT
 };
 
@@ -52,18 +59,25 @@ struct ProfSuspend {
 };
 void prof_push(int32_t kernel, int32_t variant, double flops, double bytes, hipEvent_t start, hipEvent_t stop);
 
+// `lds`: bytes of dynamic shared memory.
 template <typename Kernel, typename... Args>
-hipError_t launch(int32_t kernel_id, int32_t variant, double flops, double bytes, Kernel kernel, dim3 grid,
-                  dim3 block, hipStream_t stream, Args... args) {
+hipError_t launch_lds(int32_t kernel_id, int32_t variant, double flops, double bytes, Kernel kernel, dim3 grid,
+                      dim3 block, size_t lds, hipStream_t stream, Args... args) {
     hipEvent_t e0 = nullptr, e1 = nullptr;
     if (prof_take(&e0, &e1)) {
-        hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, e0, e1, 0, args...);
+        hipExtLaunchKernelGGL(kernel, grid, block, uint32_t(lds), stream, e0, e1, 0, args...);
         hipError_t err = hipGetLastError();
         if (err == hipSuccess) prof_push(kernel_id, variant, flops, bytes, e0, e1);
         return err;
     }
-    hipLaunchKernelGGL(kernel, grid, block, 0, stream, args...);
+    hipLaunchKernelGGL(kernel, grid, block, uint32_t(lds), stream, args...);
     return hipGetLastError();
+}
+
+template <typename Kernel, typename... Args>
+hipError_t launch(int32_t kernel_id, int32_t variant, double flops, double bytes, Kernel kernel, dim3 grid,
+                  dim3 block, hipStream_t stream, Args... args) {
+    return launch_lds(kernel_id, variant, flops, bytes, kernel, grid, block, 0, stream, args...);
 }
 
 // One launch of several that make up one record: the first carries the record's

@@ -1,0 +1,40 @@
+// Host-side validation and layout for the objectives (losses over rows of logits).
+// Pure C++ (no HIP headers), as mamw_plan.h.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "muonadamw_amd.h"
+
+namespace mamw {
+
+// Blocks of a launch over rows: each takes the rows blockIdx, blockIdx + grid, ...
+constexpr int kMaxRowBlocks = 2048;
+// Rows whose tokens one block of the counting kernel looks at where sequences do not matter.
+constexpr int kCountRows = 1024;
+// Bits of the table of a teacher's indices (128 KiB of LDS at most).
+constexpr int64_t kMaxTailVocab = int64_t(1) << 20;
+
+// A workspace: the rows that count of each sequence (or of each kCountRows rows), the length of each row's
+// sequence (policy, by sequence), the blocks' partial sums.
+struct ObjectiveWorkspace {
+    int64_t items;      // counts
+    size_t lengths_at;  // bytes from the start
+    size_t partials_at;
+    size_t bytes;
+};
+ObjectiveWorkspace objective_workspace(int64_t items, int64_t lengths, int64_t partials);
+
+int row_blocks(int64_t rows);
+
+// MAMW_OK or the first error; *ws is set where it is MAMW_OK.  `grad` may be NULL.
+int check_rows(const mamw_rows* x, const void* grad);
+int check_per_row(const mamw_per_row& a, bool needed, int32_t type, int32_t other_type = -1);
+int check_policy(const mamw_rows* x, const mamw_policy* p, const void* grad, ObjectiveWorkspace* ws);
+int check_preference(const mamw_rows* x, const mamw_preference* p, ObjectiveWorkspace* ws);
+int check_distill(const mamw_rows* x, const mamw_distill* p, const void* grad, ObjectiveWorkspace* ws);
+int check_workspace(const ObjectiveWorkspace& ws, const void* workspace, size_t bytes);
+int check_temperature(float t);
+
+}  // namespace mamw

@@ -24,6 +24,8 @@ MUON_MAX_BATCH = 32
 MUON_DIRECT_MAX = 64  # MAMW_MUON_DIRECT_MAX
 BF16_PARAM = 0x1  # MAMW_BF16_PARAM
 BF16_GRAD = 0x2   # MAMW_BF16_GRAD
+F32, BF16, F16, I32, I64, BOOL = range(6)  # MAMW_F32, ...
+MAX_TEACHER = 1024  # MAMW_MAX_TEACHER
 
 
 class AdamWTensor(ctypes.Structure):
@@ -64,6 +66,85 @@ class MuonMatrix(ctypes.Structure):
         ("cols", c_int64),
         ("scaled_lr", c_float),
         ("flags", c_int32),
+    ]
+
+
+class Rows(ctypes.Structure):
+    """``mamw_rows``."""
+
+    _fields_ = [
+        ("data", c_void_p),
+        ("outer", c_int64),
+        ("inner", c_int64),
+        ("vocab", c_int64),
+        ("outer_stride", c_int64),
+        ("inner_stride", c_int64),
+        ("type", c_int32),
+        ("reserved", c_int32),
+    ]
+
+
+class PerRow(ctypes.Structure):
+    """``mamw_per_row``."""
+
+    _fields_ = [
+        ("data", c_void_p),
+        ("outer_stride", c_int64),
+        ("inner_stride", c_int64),
+        ("type", c_int32),
+        ("reserved", c_int32),
+    ]
+
+
+class Policy(ctypes.Structure):
+    """``mamw_policy``."""
+
+    _fields_ = [
+        ("tokens", PerRow),
+        ("old_logprobs", PerRow),
+        ("advantages", PerRow),
+        ("ref_logprobs", PerRow),
+        ("offsets", c_void_p),
+        ("sequences", c_int64),
+        ("ignore_index", c_int64),
+        ("clip_low", c_float),
+        ("clip_high", c_float),
+        ("kl_coef", c_float),
+        ("temperature", c_float),
+        ("scale", c_float),
+        ("by_sequence", c_int32),
+    ]
+
+
+class Preference(ctypes.Structure):
+    """``mamw_preference``."""
+
+    _fields_ = [
+        ("tokens", PerRow),
+        ("ref_logprobs", c_void_p),
+        ("offsets", c_void_p),
+        ("sequences", c_int64),
+        ("ignore_index", c_int64),
+        ("beta", c_float),
+        ("smoothing", c_float),
+        ("temperature", c_float),
+        ("kind", c_int32),
+        ("length_average", c_int32),
+        ("reserved", c_int32),
+    ]
+
+
+class Distill(ctypes.Structure):
+    """``mamw_distill``."""
+
+    _fields_ = [
+        ("teacher_logits", PerRow),
+        ("teacher_indices", PerRow),
+        ("teacher_lse", PerRow),
+        ("mask", PerRow),
+        ("k", c_int64),
+        ("temperature", c_float),
+        ("scale", c_float),
     ]
 
 
@@ -134,6 +215,39 @@ _PROTOTYPES = {
     "mamw_ns_direct": (
         c_int,
         [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_float, c_float, c_void_p, c_size_t, c_void_p],
+    ),
+    "mamw_token_logprobs": (
+        c_int,
+        [POINTER(Rows), POINTER(PerRow), c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "mamw_logits_grad": (
+        c_int,
+        [POINTER(Rows), POINTER(PerRow), c_int64, c_float, c_void_p, POINTER(PerRow), POINTER(PerRow), c_void_p,
+         c_void_p, c_void_p, c_void_p],
+    ),
+    "mamw_policy_workspace_bytes": (c_int, [POINTER(Rows), POINTER(Policy), POINTER(c_size_t)]),
+    "mamw_policy_loss": (
+        c_int,
+        [POINTER(Rows), POINTER(Policy), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "mamw_policy_grad": (
+        c_int,
+        [POINTER(Rows), POINTER(Policy), c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "mamw_preference_workspace_bytes": (c_int, [POINTER(Rows), POINTER(Preference), POINTER(c_size_t)]),
+    "mamw_preference_loss": (
+        c_int,
+        [POINTER(Rows), POINTER(Preference), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+         c_void_p],
+    ),
+    "mamw_distill_workspace_bytes": (c_int, [POINTER(Rows), POINTER(Distill), POINTER(c_size_t)]),
+    "mamw_distill_loss": (
+        c_int,
+        [POINTER(Rows), POINTER(Distill), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "mamw_distill_grad": (
+        c_int,
+        [POINTER(Rows), POINTER(Distill), c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
     "mamw_prof_start": (c_int, []),
     "mamw_prof_stop": (c_int, []),
