@@ -331,7 +331,7 @@ int mamw_ns_direct(int op, const uint16_t* X, const uint16_t* S, uint16_t* out,
 typedef struct mamw_rows {
     const void* data;
     int64_t     outer, inner;  /* >= 0, their product below 2^31 */
-    int64_t     vocab;         /* 1 .. 2^31 - 1                   */
+    int64_t     vocab;         /* 1 .. 2^30                       */
     int64_t     outer_stride, inner_stride;
     int32_t     type;          /* MAMW_F32, MAMW_BF16 or MAMW_F16 */
     int32_t     reserved;      /* must be 0                       */

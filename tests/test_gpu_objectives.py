@@ -443,10 +443,18 @@ def layout_inputs(vocab, dtype):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("vocab", [33, 1003, 9001, 50257, 70001])
 def test_strides_and_alignment_change_nothing(gpu, dtype, vocab):
-    """Padded and offset vocabularies, swapped dimensions, steps, broadcast rows: the same bits as dense inputs."""
+    """Padded and offset vocabularies, swapped dimensions, steps.  Which thread adds which logit goes by the row's
+    place in memory, so results are equal to within their tolerance on either side: a log-probability's d, with
+    values and gradients of order 1 here, and a place of the type."""
     dense = layout_inputs(vocab, dtype)
     expect = everything(*dense)
     x = dense[0]
+    d = 16 * lp_tol(vocab, 40.0)
+
+    def same(got, label):
+        for i, (p, q) in enumerate(zip(got, expect)):
+            off = np.abs(f64(p) - f64(q)) - (d * np.maximum(1.0, np.abs(f64(q))) + 2 * HALF_PLACE[q.dtype] * np.abs(f64(q)))
+            assert off.max() <= 0, (label, i, off.max())
 
     def padded(v, left, right):
         wide = torch.full((*v.shape[:-1], v.shape[-1] + left + right), float("nan") if v.is_floating_point() else 1,
@@ -462,14 +470,11 @@ def test_strides_and_alignment_change_nothing(gpu, dtype, vocab):
         return wide[:, ::2]
 
     for change in (lambda v: padded(v, 0, 7), lambda v: padded(v, 1, 2), lambda v: padded(v, 3, 64), swapped, stepped):
-        got = everything(change(x), *[change(v) if v.dim() == 3 else swapped(v) for v in dense[1:]])
-        for i, (p, q) in enumerate(zip(got, expect)):
-            assert torch.equal(p, q), i
+        same(everything(change(x), *[change(v) if v.dim() == 3 else swapped(v) for v in dense[1:]]), change)
     # logits that start off the 16-byte boundary
     flat = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
     flat[1:] = x.flatten()
-    for p, q in zip(everything(flat[1:].view(x.shape), *dense[1:]), expect):
-        assert torch.equal(p, q)
+    same(everything(flat[1:].view(x.shape), *dense[1:]), "offset")
 
 
 def test_broadcast_logits(gpu):
@@ -484,7 +489,8 @@ def test_broadcast_logits(gpu):
 
 @pytest.mark.parametrize("dtype", ["bf16"])
 def test_offsets_beyond_32_bits(gpu, dtype):
-    """Rows more than 2^31 elements and 2^32 bytes apart."""
+    """Rows more than 2^31 elements and 2^32 bytes apart; off the 16-byte boundary where the near ones are on it, so
+    to within the tolerance on either side (values of order 1)."""
     vocab, stride = 1003, (1 << 31) + 9
     flat = torch.empty(2 * stride + vocab, dtype=DTYPES[dtype], device="cuda")
     x, tokens, gen = make(3, vocab, dtype, 33, ignored=0.0)
@@ -492,9 +498,10 @@ def test_offsets_beyond_32_bits(gpu, dtype):
     far.copy_(x)
     old, adv = normal(3, 1.0, gen) - 4, normal(3, 1.0, gen)
     with torch.no_grad():
-        for a, b in zip(policy_loss(far, tokens, old, adv), policy_loss(x, tokens, old, adv)):
-            assert torch.equal(a, b)
-        assert torch.equal(token_logprobs(far, tokens), token_logprobs(x, tokens))
+        pairs = [*zip(policy_loss(far, tokens, old, adv), policy_loss(x, tokens, old, adv)),
+                 (token_logprobs(far, tokens), token_logprobs(x, tokens))]
+    for a, b in pairs:
+        assert (np.abs(f64(a) - f64(b)) <= 16 * lp_tol(vocab, f64(b)) * np.maximum(1.0, np.abs(f64(b)))).all()
 
 
 def test_gradient_beyond_32_bits(gpu):

@@ -9,15 +9,13 @@
 
 namespace mamw {
 
-// Blocks of a launch over rows: each takes the rows blockIdx, blockIdx + grid, ...
-constexpr int kMaxRowBlocks = 2048;
 // Rows whose tokens one block of the counting kernel looks at where sequences do not matter.
 constexpr int kCountRows = 1024;
 // Bits of the table of a teacher's indices (128 KiB of LDS at most).
 constexpr int64_t kMaxTailVocab = int64_t(1) << 20;
 
 // A workspace: the rows that count of each sequence (or of each kCountRows rows), the length of each row's
-// sequence (policy, by sequence), the blocks' partial sums.
+// sequence (policy, by sequence), the rows' parts of the result.
 struct ObjectiveWorkspace {
     int64_t items;      // counts
     size_t lengths_at;  // bytes from the start
@@ -25,8 +23,6 @@ struct ObjectiveWorkspace {
     size_t bytes;
 };
 ObjectiveWorkspace objective_workspace(int64_t items, int64_t lengths, int64_t partials);
-
-int row_blocks(int64_t rows);
 
 // MAMW_OK or the first error; *ws is set where it is MAMW_OK.  `grad` may be NULL.
 int check_rows(const mamw_rows* x, const void* grad);

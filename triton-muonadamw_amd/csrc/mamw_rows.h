@@ -1,0 +1,533 @@
+// Device side of the objectives' kernels over rows of logits: element types, where a row and what goes with it lie,
+// the statistics of its softmax, and a row held in registers.
+#pragma once
+
+#include "mamw_device.h"
+#include "mamw_launch.h"
+#include "mamw_objectives.h"
+
+namespace mamw {
+
+constexpr int kThreads = 256;  // of the kernels that are not over logits
+constexpr int kWaves = kThreads / 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kSmallestTail = 0x1p-20f;
+
+// ---- element types
+
+struct bf16_t {
+    uint16_t bits;
+};
+
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(bf16_t x) { return bf16_to_f32(x.bits); }
+__device__ __forceinline__ float widen(_Float16 x) { return float(x); }
+
+template <typename T>
+__device__ __forceinline__ T narrow(float x);  // to nearest, ties to even
+template <>
+__device__ __forceinline__ float narrow<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16_t narrow<bf16_t>(float x) { return {uint16_t(f32_to_bf16(x))}; }
+template <>
+__device__ __forceinline__ _Float16 narrow<_Float16>(float x) { return _Float16(x); }
+
+// 16 bytes of a row: kVec<T> elements.
+typedef uint32_t vec_t __attribute__((ext_vector_type(4)));
+typedef vec_t any_vec_t __attribute__((aligned(2)));  // at any element
+template <typename T>
+constexpr int kVec = int(16 / sizeof(T));
+
+template <typename T>
+__device__ __forceinline__ void unpack(vec_t v, float* f) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(v[i]);
+    } else if constexpr (__is_same(T, bf16_t)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(v[i] << 16);
+            f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = float(__builtin_bit_cast(_Float16, uint16_t(v[i] & 0xffffu)));
+            f[2 * i + 1] = float(__builtin_bit_cast(_Float16, uint16_t(v[i] >> 16)));
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ vec_t pack(const float* f) {
+    vec_t v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4)
+            v[i] = __float_as_uint(f[i]);
+        else if constexpr (__is_same(T, bf16_t))
+            v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+        else
+            v[i] = uint32_t(__builtin_bit_cast(uint16_t, _Float16(f[2 * i]))) |
+                   uint32_t(__builtin_bit_cast(uint16_t, _Float16(f[2 * i + 1]))) << 16;
+    }
+    return v;
+}
+
+// Elements of no probability.
+template <typename T>
+__device__ __forceinline__ vec_t nothing() {
+    const uint32_t w = sizeof(T) == 4 ? 0xff800000u : __is_same(T, bf16_t) ? 0xff80ff80u : 0xfc00fc00u;
+    return {w, w, w, w};
+}
+
+// ---- what the kernels are given
+
+struct Rows {
+    const char* data;
+    int64_t outer_stride, inner_stride;
+    uint32_t inner;
+    int32_t rows, vocab;
+    float c, inv_t;  // log2(e) / T, 1 / T
+};
+
+struct PerRow {
+    const char* data;
+    int64_t outer_stride, inner_stride;
+    int32_t type;
+};
+
+struct Place {
+    uint32_t outer, inner;
+};
+
+// Row r is the same for the whole workgroup; so that addresses made of it stay in scalar registers, the quotient, which
+// the vector unit forms, is brought back there.
+__device__ __forceinline__ Place place(const Rows& x, uint32_t r) {
+    const uint32_t o = __builtin_amdgcn_readfirstlane(r / x.inner);
+    return {o, r - o * x.inner};
+}
+__device__ __forceinline__ uint32_t row_of_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+// The same for rows that differ between threads.
+__device__ __forceinline__ Place place_of_thread(const Rows& x, uint32_t r) {
+    const uint32_t o = r / x.inner;
+    return {o, r - o * x.inner};
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const Rows& x, Place at) {
+    return reinterpret_cast<const T*>(x.data) + (at.outer * x.outer_stride + at.inner * x.inner_stride);
+}
+
+__device__ __forceinline__ int64_t offset(const PerRow& a, Place at) {
+    return at.outer * a.outer_stride + at.inner * a.inner_stride;
+}
+__device__ __forceinline__ float load_f32(const PerRow& a, Place at) {
+    return reinterpret_cast<const float*>(a.data)[offset(a, at)];
+}
+__device__ __forceinline__ int64_t load_int(const PerRow& a, int64_t i) {
+    return a.type == MAMW_I32 ? int64_t(reinterpret_cast<const int32_t*>(a.data)[i])
+                              : reinterpret_cast<const int64_t*>(a.data)[i];
+}
+__device__ __forceinline__ bool load_mask(const PerRow& a, Place at) {
+    return !a.data || reinterpret_cast<const uint8_t*>(a.data)[offset(a, at)] != 0;
+}
+
+struct Sequences {
+    const int64_t* offsets;
+    int64_t count;
+};
+
+// ---- reductions over the workgroup, always in the same order
+
+template <int N>
+struct Floats {
+    float v[N];
+};
+
+template <int N, int kThreads_ = kThreads>
+__device__ __forceinline__ Floats<N> block_sum(Floats<N> x, float* lds) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = wave_sum(x.v[i]);
+    const int wave = threadIdx.x / 64;
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) lds[wave * N + i] = x.v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x.v[i] = lds[i];
+        for (int w = 1; w < kThreads_ / 64; ++w) x.v[i] += lds[w * N + i];
+    }
+    return x;
+}
+
+// ---- a row
+
+// y_j = log2 of exp((x_j - m) / T).  The difference first: logits and masks may be the type's lowest value, whose
+// product with log2(e) / T overflows (the fused form, one operation less, is no faster: 399 against 401 us for
+// 4096 x 128256 bf16).
+__device__ __forceinline__ float below(float x, float m, float c) { return (x - m) * c; }
+
+// A row as `vecs` vectors on 16-byte boundaries, from element `head` on, and `extra` single elements before and after
+// them.  Loads that straddle the boundary cost: 8192 x 50257 bf16 with its odd rows took 162 us to read, against 117
+// for as many bytes on the boundary.
+struct Span {
+    int head, vecs, extra;
+};
+
+template <typename T>
+__device__ __forceinline__ Span span_of(const T* row, int vocab) {
+    Span s;
+    s.head = min(vocab, int((-reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)));
+    s.vecs = (vocab - s.head) / kVec<T>;
+    s.extra = s.head + (vocab - s.head) % kVec<T>;
+    return s;
+}
+
+// The element of single element e < extra.
+template <typename T>
+__device__ __forceinline__ int extra_element(const Span& s, int e) {
+    return e < s.head ? e : e + s.vecs * kVec<T>;
+}
+
+// The thread of `threads` that writes element j, where vector n is thread n % threads' and single element e thread e's.
+template <typename T>
+__device__ __forceinline__ int owner_of(const Span& s, int j, int threads) {
+    if (j < s.head) return j;
+    const int n = (j - s.head) / kVec<T>;
+    return n < s.vecs ? n % threads : j - s.vecs * kVec<T>;
+}
+
+// Rows pass through once: kept out of the caches' way (4096 x 128256 bf16, read and written: 399 us without, 375
+// with).
+//
+// Vector `thread` of those from `first` on, with `first` the same for the whole workgroup: scalar address and 32-bit
+// offset, no registers for sixteen 64-bit addresses.
+__device__ __forceinline__ vec_t load_vec(const void* vecs, int first, int thread) {
+    const char* at = static_cast<const char*>(vecs) + int64_t(first) * 16;
+    return __builtin_nontemporal_load(reinterpret_cast<const vec_t*>(at + uint32_t(thread) * 16u));
+}
+__device__ __forceinline__ void store_vec(void* vecs, int first, int thread, vec_t v) {
+    // at any element: the gradient's rows may lie otherwise than the logits'
+    char* at = static_cast<char*>(vecs) + int64_t(first) * 16;
+    __builtin_nontemporal_store(v, reinterpret_cast<any_vec_t*>(at + uint32_t(thread) * 16u));
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_row(T* __restrict__ g, int vocab, int threads) {
+    const Span s = span_of(g, vocab);
+    const int t = threadIdx.x;
+    for (int n = 0; n + t < s.vecs; n += threads) store_vec(g + s.head, n, t, vec_t{0, 0, 0, 0});
+    if (int(threadIdx.x) < s.extra) g[extra_element<T>(s, threadIdx.x)] = narrow<T>(0.f);
+}
+
+// The logit of the row's token: NaN where it is beyond the vocabulary.
+template <typename T>
+__device__ __forceinline__ float chosen(const T* x, int64_t token, int vocab) {
+    return token >= 0 && token < vocab ? widen(x[token]) : NAN;
+}
+
+// Running softmax statistics: the largest logit m so far, s = sum of 2^y and sy = sum of 2^y y (entropies) below it.
+struct Stats {
+    float m, s, sy;
+};
+__device__ __forceinline__ Stats no_stats() { return {-INFINITY, 0.f, 0.f}; }
+
+__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
+
+// st as seen from a larger m.
+template <bool kEntropy>
+__device__ __forceinline__ void move_to(Stats& st, float m, float c) {
+    const float y = fmaxf(below(st.m, reference(m), c), -1e30f);  // finite: times s = 0 it is 0
+    const float f = __builtin_amdgcn_exp2f(y);
+    if (kEntropy) st.sy = f * (st.sy + y * st.s);
+    st.s *= f;
+    st.m = m;
+}
+
+template <bool kEntropy>
+__device__ __forceinline__ void add(Stats& st, float x, float ref, float c) {
+    const float y = below(x, ref, c), e = __builtin_amdgcn_exp2f(y);
+    st.s += e;
+    if (kEntropy) st.sy += e * fmaxf(y, -1e30f);  // 0 * -inf: entries of no probability add nothing
+}
+
+// kCount vectors more.
+template <typename T, bool kEntropy, int kCount>
+__device__ __forceinline__ void add_vecs(Stats& st, const vec_t* v, float c) {
+    float m = st.m;
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+        float f[kVec<T>];
+        unpack<T>(v[u], f);
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, f[k]);
+    }
+    move_to<kEntropy>(st, m, c);
+    const float ref = reference(m);
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+        float f[kVec<T>];
+        unpack<T>(v[u], f);
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) add<kEntropy>(st, f[k], ref, c);
+    }
+}
+
+// The statistics of vectors from + threadIdx.x, + kThreads_, ... below `to`; change(v, n) is applied to vector n.
+template <typename T, bool kEntropy, int kThreads_, typename Change>
+__device__ __forceinline__ void read_vecs(Stats& st, const void* vecs, int from, int to, float c, Change change) {
+    constexpr int kUnroll = 4;
+    const int t = threadIdx.x;
+    int n = from;
+    for (; n + kUnroll * kThreads_ <= to; n += kUnroll * kThreads_) {
+        vec_t v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_vec(vecs, n + u * kThreads_, t);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) change(v[u], n + u * kThreads_ + t);
+        add_vecs<T, kEntropy, kUnroll>(st, v, c);
+    }
+    for (; n + t < to; n += kThreads_) {
+        vec_t v[1] = {load_vec(vecs, n, t)};
+        change(v[0], n + t);
+        add_vecs<T, kEntropy, 1>(st, v, c);
+    }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+
+template <bool kEntropy>
+__device__ __forceinline__ Stats over_wave(Stats st, float c) {
+    move_to<kEntropy>(st, wave_max(st.m), c);
+    st.s = wave_sum(st.s);
+    if (kEntropy) st.sy = wave_sum(st.sy);
+    return st;
+}
+
+// The workgroup's statistics from its waves', through `lds` (one a wave).  One barrier, between writing and reading.
+template <bool kEntropy, int kThreads_>
+__device__ __forceinline__ Stats over_block(const Stats& wave, float c, Stats* lds) {
+    constexpr int kN = kThreads_ / 64;
+    Stats st = wave;
+    if constexpr (kN > 1) {
+        if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = wave;
+        __syncthreads();
+        st = lds[threadIdx.x % kN];
+    }
+    float m = st.m;
+#pragma unroll
+    for (int o = kN / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    move_to<kEntropy>(st, m, c);
+#pragma unroll
+    for (int o = kN / 2; o >= 1; o >>= 1) {
+        st.s += __shfl_xor(st.s, o, 64);
+        if (kEntropy) st.sy += __shfl_xor(st.sy, o, 64);
+    }
+    return st;
+}
+
+// A row in the registers of a workgroup: vector i kThreads + t of the row is v[i] of thread t, single element t its
+// `single`.  Rows longer than that (kRest) have their remaining vectors read twice.
+template <typename T, int kThreads_, int kVecs, bool kRest>
+struct HeldRow {
+    const T* row;
+    Span span;
+    vec_t v[kVecs];
+    float single;
+    float wave_ref;  // float: v holds 2^y below this, once the statistics are taken
+
+    __device__ __forceinline__ const void* vecs() const { return row + span.head; }
+
+    __device__ __forceinline__ void load(const T* row_, int vocab) {
+        row = row_;
+        span = span_of(row_, vocab);
+        if constexpr (!kRest) load_held();
+        single = int(threadIdx.x) < span.extra ? widen(row_[extra_element<T>(span, threadIdx.x)]) : -INFINITY;
+    }
+
+    __device__ __forceinline__ void load_held() {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int n = i * kThreads_;
+            v[i] = n + int(threadIdx.x) < span.vecs ? load_vec(vecs(), n, threadIdx.x) : nothing<T>();
+        }
+    }
+
+    // fn(vector, its number less threadIdx.x) for each held one in turn.  The empty statement keeps the compiler from
+    // unpacking all of them once and for both passes, which takes twice the registers.
+    template <typename Fn>
+    __device__ __forceinline__ void each(Fn fn) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+            if (i * kThreads_ < span.vecs) {
+                asm volatile("" : "+v"(v[i]));
+                fn(v[i], i * kThreads_);
+            }
+    }
+
+    // The wave's statistics.  change(vector, number) is for the vectors that are not held, and with kRest for all: those
+    // held are loaded last then, for the registers.
+    template <typename Change>
+    __device__ __forceinline__ Stats stats(float c, Change change) {
+        Stats st = no_stats();
+        if constexpr (kRest) {
+            read_vecs<T, false, kThreads_>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
+            load_held();
+            each([&](vec_t& x, int n) { change(x, n + int(threadIdx.x)); });
+        }
+        float m = fmaxf(st.m, single);
+        each([&](vec_t& x, int) {
+            float f[kVec<T>];
+            unpack<T>(x, f);
+#pragma unroll
+            for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, f[k]);
+        });
+        move_to<false>(st, wave_max(m), c);
+        const float ref = wave_ref = reference(st.m);
+        add<false>(st, single, ref, c);
+        each([&](vec_t& x, int) {
+            float f[kVec<T>];
+            unpack<T>(x, f);
+#pragma unroll
+            for (int k = 0; k < kVec<T>; ++k) {
+                f[k] = __builtin_amdgcn_exp2f(below(f[k], ref, c));
+                st.s += f[k];
+            }
+            if constexpr (sizeof(T) == 4) x = pack<T>(f);
+        });
+        st.s = wave_sum(st.s);
+        return st;
+    }
+
+    // g_j = b 2^y below m.
+    template <typename Change>
+    __device__ __forceinline__ void write(T* __restrict__ g, float b, float m, float c, Change change) {
+        const float from_wave = b * __builtin_amdgcn_exp2f(below(wave_ref, m, c));
+        T* at = g + span.head;
+        const int t = threadIdx.x;
+        each([&](vec_t& x, int n) {
+            float f[kVec<T>];
+            unpack<T>(x, f);
+#pragma unroll
+            for (int k = 0; k < kVec<T>; ++k)
+                f[k] = sizeof(T) == 4 ? from_wave * f[k] : b * __builtin_amdgcn_exp2f(below(f[k], m, c));
+            if (n + t < span.vecs) store_vec(at, n, t, pack<T>(f));
+        });
+        if constexpr (kRest) {
+            constexpr int kUnroll = 4;
+            for (int n = kVecs * kThreads_; n < span.vecs; n += kUnroll * kThreads_) {
+                vec_t x[kUnroll];
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    const int first = n + u * kThreads_;
+                    x[u] = first + t < span.vecs ? load_vec(vecs(), first, t) : nothing<T>();
+                }
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    const int first = n + u * kThreads_;
+                    change(x[u], first + t);
+                    float f[kVec<T>];
+                    unpack<T>(x[u], f);
+#pragma unroll
+                    for (int k = 0; k < kVec<T>; ++k) f[k] = b * __builtin_amdgcn_exp2f(below(f[k], m, c));
+                    if (first + t < span.vecs) store_vec(at, first, t, pack<T>(f));
+                }
+            }
+        }
+        if (t < span.extra)
+            g[extra_element<T>(span, threadIdx.x)] = narrow<T>(b * __builtin_amdgcn_exp2f(below(single, m, c)));
+    }
+};
+
+struct Unchanged {
+    __device__ __forceinline__ void operator()(vec_t&, int) const {}
+};
+
+// The number that weights are divided by: rows that count, or sequences that have any.  Every wave by itself.
+__device__ __forceinline__ float count_all(const int32_t* __restrict__ count, int64_t items, bool by_sequence) {
+    float n = 0.f;
+    for (int64_t i = threadIdx.x % 64; i < items; i += 64) n += by_sequence ? float(count[i] > 0) : float(count[i]);
+    return fmaxf(wave_sum(n), 1.f);
+}
+
+// ---- launches
+
+// Waves that should fit a SIMD beside each other: 512 registers shared among them, kVecs * 4 a wave for the row and
+// some 40 to 60 for the rest.
+template <int kVecs>
+constexpr int kRowWaves = kVecs > 8 ? 4 : kVecs > 4 ? 5 : kVecs > 2 ? 6 : 8;
+
+inline Rows make_rows(const mamw_rows& x, float temperature) {
+    Rows r;
+    r.data = static_cast<const char*>(x.data);
+    r.outer_stride = x.outer_stride;
+    r.inner_stride = x.inner_stride;
+    r.inner = uint32_t(x.inner);
+    r.rows = int32_t(x.outer * x.inner);
+    r.vocab = int32_t(x.vocab);
+    r.c = kLog2e / temperature;
+    r.inv_t = 1.f / temperature;
+    return r;
+}
+
+inline PerRow make_per_row(const mamw_per_row& a) {
+    return {static_cast<const char*>(a.data), a.outer_stride, a.inner_stride, a.type};
+}
+
+// fn(element type): the logits' type as a type.
+template <typename Fn>
+int with_type(int32_t type, Fn fn) {
+    switch (type) {
+        case MAMW_F32: return fn(float());
+        case MAMW_BF16: return fn(bf16_t());
+        default: return fn(_Float16());
+    }
+}
+
+inline double row_bytes(const mamw_rows& x, bool grad) {
+    return double(x.outer * x.inner) * double(x.vocab) * (x.type == MAMW_F32 ? 4.0 : 2.0) * (grad ? 2.0 : 1.0);
+}
+
+// fn(workgroup size, vectors a thread, whether some are left) for rows of `vecs` vectors, held by one workgroup.
+// Each thread keeps one to sixteen: fewer threads of more would leave the reductions to fewer waves, and a row of 256
+// KiB is all the registers of a compute unit that its other values leave.  A longer row keeps 224 KiB and has the rest
+// read twice.
+template <int kN>
+struct Int {
+    static constexpr int value = kN;
+};
+template <typename Fn>
+int with_held_row(int64_t vecs, Fn fn) {
+    if (vecs <= 256) return fn(Int<256>(), Int<1>(), Int<0>());
+    if (vecs <= 512) return fn(Int<256>(), Int<2>(), Int<0>());
+    if (vecs <= 1024) return fn(Int<256>(), Int<4>(), Int<0>());
+    if (vecs <= 2048) return fn(Int<256>(), Int<8>(), Int<0>());
+    if (vecs <= 4096) return fn(Int<512>(), Int<8>(), Int<0>());
+    if (vecs <= 8192) return fn(Int<512>(), Int<16>(), Int<0>());
+    if (vecs <= 16384) return fn(Int<1024>(), Int<16>(), Int<0>());
+    return fn(Int<1024>(), Int<14>(), Int<1>());
+}
+
+// One workgroup a row.  Such workgroups come and go by themselves: a row's loads do not wait for the stores of the row
+// before, as they would in a loop over rows, where the same counter covers both (65536 x 4096 bf16: 205 us in 2048
+// workgroups, 180 in 65536).
+inline dim3 row_grid(int64_t rows) {
+    const unsigned most = 1u << 16;
+    return rows <= int64_t(most) ? dim3(unsigned(rows)) : dim3(most, unsigned((rows + most - 1) / most));
+}
+
+// Defined in objectives.hip.
+int launch_count(const Rows& rows, const PerRow& tokens, int64_t ignore, const PerRow& mask, const Sequences& seqs,
+                 const ObjectiveWorkspace& ws, bool by_sequence, char* base, hipStream_t stream);
+int launch_result(const ObjectiveWorkspace& ws, char* base, int64_t rows, float f, float* result, hipStream_t stream);
+
+}  // namespace mamw

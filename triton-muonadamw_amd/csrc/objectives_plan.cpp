@@ -3,8 +3,6 @@
 
 #include <math.h>
 
-#include <algorithm>
-
 #include "mamw_plan.h"
 
 namespace mamw {
@@ -36,13 +34,11 @@ ObjectiveWorkspace objective_workspace(int64_t items, int64_t lengths, int64_t p
     return w;
 }
 
-int row_blocks(int64_t rows) { return int(std::min<int64_t>(rows, kMaxRowBlocks)); }
-
 int check_rows(const mamw_rows* x, const void* grad) {
     if (!x) return MAMW_ERR_NULL;
     if (x->type != MAMW_F32 && x->type != MAMW_BF16 && x->type != MAMW_F16) return MAMW_ERR_HYPER;
     if (x->reserved) return MAMW_ERR_HYPER;
-    if (x->outer < 0 || x->inner < 0 || x->vocab < 1 || x->vocab > int64_t(0x7fffffff)) return MAMW_ERR_SHAPE;
+    if (x->outer < 0 || x->inner < 0 || x->vocab < 1 || x->vocab > int64_t(1) << 30) return MAMW_ERR_SHAPE;
     if (x->outer_stride < 0 || x->inner_stride < 0) return MAMW_ERR_SHAPE;
     const int64_t most = int64_t(0x7fffffff);
     if (x->outer > most || x->inner > most || x->outer * x->inner > most) return MAMW_ERR_COUNT;
@@ -104,8 +100,8 @@ int check_policy(const mamw_rows* x, const mamw_policy* p, const void* grad, Obj
     if ((st = check_temperature(p->temperature)) != MAMW_OK) return st;
     if (!(p->clip_low >= 0.f) || !(p->clip_high >= 0.f) || !isfinite(p->kl_coef) || !isfinite(p->scale))
         return MAMW_ERR_HYPER;
-    *ws = p->by_sequence ? objective_workspace(p->sequences, rows, 4 * kMaxRowBlocks)
-                         : objective_workspace(count_items(rows), 0, 4 * kMaxRowBlocks);
+    *ws = p->by_sequence ? objective_workspace(p->sequences, rows, 4 * rows)
+                         : objective_workspace(count_items(rows), 0, 4 * rows);
     return MAMW_OK;
 }
 
@@ -144,7 +140,7 @@ int check_distill(const mamw_rows* x, const mamw_distill* p, const void* grad, O
     if ((st = check_temperature(p->temperature)) != MAMW_OK) return st;
     if (!isfinite(p->scale)) return MAMW_ERR_HYPER;
     if (p->teacher_lse.data && x->vocab > kMaxTailVocab) return MAMW_ERR_SHAPE;
-    *ws = objective_workspace(count_items(rows), 0, 4 * kMaxRowBlocks);
+    *ws = objective_workspace(count_items(rows), 0, 4 * rows);
     return MAMW_OK;
 }
 

@@ -34,7 +34,7 @@ LAYOUT_PATH = PKG_DIR / ("_layout" + sysconfig.get_config_var("EXT_SUFFIX"))
 ARCH = "gfx950"
 
 SOURCES = ["mamw_plan.cpp", "abi.cpp", "prof.cpp", "adamw.hip", "muon.hip", "muon_direct.hip",
-           "objectives_plan.cpp", "objectives.hip"]
+           "objectives_plan.cpp", "objectives.hip", "objective_policy.hip", "objective_distill.hip"]
 
 COMMON_FLAGS = [
     "-O3",
