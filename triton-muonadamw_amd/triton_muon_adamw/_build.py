@@ -31,6 +31,9 @@ LIB_PATH = PKG_DIR / LIB_NAME
 # CPython module (csrc/layout.cpp), see _lib.layout; the suffix names the Python it is for.
 LAYOUT_PATH = PKG_DIR / ("_layout" + sysconfig.get_config_var("EXT_SUFFIX"))
 
+# CPython module (csrc/objectives_module.cpp), see _lib.objectives; linked against LIB_PATH.
+OBJECTIVES_PATH = LAYOUT_PATH.with_name("_objectives" + sysconfig.get_config_var("EXT_SUFFIX"))
+
 ARCH = "gfx950"
 
 SOURCES = ["mamw_plan.cpp", "abi.cpp", "prof.cpp", "adamw.hip", "muon.hip", "muon_direct.hip",
@@ -134,22 +137,21 @@ def _check_untracked_reads(src: Path, verbose: bool, out_dir: Path = BUILD_DIR) 
                            + "\n".join(rep.hazards[:20]))
 
 
-def _build_layout(verbose: bool) -> None:
-    """The CPython module: host C++ against torch's and Python's headers (no HIP).
-    Without it the package runs all the same (``_lib.layout``), so a host that
-    cannot compile it gets a warning."""
+def _build_module(source: str, path: Path, verbose: bool, *more: str) -> str:
+    """Compile a CPython module, host C++ against torch's and Python's headers;
+    returns why it failed, or nothing."""
     import torch
     from torch.utils.cpp_extension import include_paths
 
-    LAYOUT_PATH.unlink(missing_ok=True)  # an older one may not be this torch's
+    path.unlink(missing_ok=True)  # an older one may not be this torch's
     lib_dir = Path(torch.__file__).resolve().parent / "lib"
     cxx = (os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
            or str(Path(_hipcc()).with_name("amdclang++")))
-    tmp = LAYOUT_PATH.with_name(LAYOUT_PATH.name + ".tmp")
+    tmp = path.with_name(path.name + ".tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{d}" for d in include_paths()), f"-I{sysconfig.get_paths()['include']}",
-           str(CSRC / "layout.cpp"), f"-L{lib_dir}", "-lc10", "-ltorch_cpu", "-ltorch_python", "-o", str(tmp)]
+           str(CSRC / source), f"-L{lib_dir}", "-lc10", "-ltorch_cpu", "-ltorch_python", *more, "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)
     try:
@@ -157,11 +159,30 @@ def _build_layout(verbose: bool) -> None:
         failed = res.returncode != 0 and f"\n{res.stdout}\n{res.stderr}"
     except OSError as e:
         failed = f" {e}"
+    if not failed:
+        os.replace(tmp, path)
+    return failed or ""
+
+
+def _build_layout(verbose: bool) -> None:
+    """Without this module the package runs all the same (``_lib.layout``), so a
+    host that cannot compile it gets a warning."""
+    failed = _build_module("layout.cpp", LAYOUT_PATH, verbose)
     if failed:
         warnings.warn("triton_muon_adamw._layout was not built: optimizer steps will compare their launch plans "
                       f"in Python (about 1 us a parameter).{failed}", RuntimeWarning, stacklevel=2)
-        return
-    os.replace(tmp, LAYOUT_PATH)
+
+
+def _build_objectives(verbose: bool) -> None:
+    """The objectives' torch calls, linked against the library beside them.  The
+    optimizer does not need them, so here, too, a failure is a warning; calling
+    an objective raises then (``_lib.objectives``)."""
+    failed = _build_module("objectives_module.cpp", OBJECTIVES_PATH, verbose, f"-I{INCLUDE}", "-I/opt/rocm/include",
+                           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-lc10_hip", f"-L{PKG_DIR}", f"-l:{LIB_NAME}",
+                           "-Wl,-rpath,$ORIGIN")
+    if failed:
+        warnings.warn(f"triton_muon_adamw._objectives was not built: the objectives cannot be used.{failed}",
+                      RuntimeWarning, stacklevel=2)
 
 
 def build(verbose: bool = False) -> Path:
@@ -188,6 +209,7 @@ def build(verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
+    _build_objectives(verbose)
     return LIB_PATH
 
 

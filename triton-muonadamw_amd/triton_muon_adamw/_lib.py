@@ -354,6 +354,28 @@ def layout(params) -> tuple[list, object]:
     return found
 
 
+_objectives = None
+
+
+def objectives():
+    """The native module of the objectives (``csrc/objectives_module.cpp``).
+    There is no other path: where it is not built for this Python and torch,
+    calling an objective raises."""
+    global _objectives
+    if _objectives is None:
+        load()
+        try:
+            from . import _objectives as module
+            why = module.torch_version != torch.__version__.split("+")[0] and f"built with torch {module.torch_version}"
+        except ImportError as e:
+            why = str(e)
+        if why:
+            raise RuntimeError(f"triton_muon_adamw._objectives cannot be used ({why}); run __graft_entry__.build() "
+                               "(or python -m triton_muon_adamw._build).")
+        _objectives = module
+    return _objectives
+
+
 def check_not_capturing(branch: str) -> None:
     """Launch plans and device step counters are made by eager steps only: a
     graph replays the pointers, scalars and table upload recorded at capture."""
