@@ -256,8 +256,10 @@ __device__ __forceinline__ void add(Stats& st, float x, float ref, float c) {
     if (kEntropy) st.sy += e * fmaxf(y, -1e30f);  // 0 * -inf: entries of no probability add nothing
 }
 
-// kCount vectors more.
-template <typename T, bool kEntropy, int kCount>
+// kCount vectors more.  kQuick: two operations an element less, of eleven, with y = x c - m c in one and without the
+// guard of entropies; not finite, or nothing, where m c overflows or an entry is -inf (see quick_holds).  What the
+// rounding of m c has moved all y by is put right in the sums.
+template <typename T, bool kEntropy, bool kQuick, int kCount>
 __device__ __forceinline__ void add_vecs(Stats& st, const vec_t* v, float c) {
     float m = st.m;
 #pragma unroll
@@ -268,35 +270,65 @@ __device__ __forceinline__ void add_vecs(Stats& st, const vec_t* v, float c) {
         for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, f[k]);
     }
     move_to<kEntropy>(st, m, c);
-    const float ref = reference(m);
+    const float ref = reference(m), shift = -ref * c;
+    float s = 0.f, sy = 0.f;
 #pragma unroll
     for (int u = 0; u < kCount; ++u) {
         float f[kVec<T>];
         unpack<T>(v[u], f);
 #pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) add<kEntropy>(st, f[k], ref, c);
+        for (int k = 0; k < kVec<T>; ++k) {
+            if constexpr (kQuick) {
+                const float y = __builtin_fmaf(f[k], c, shift), e = __builtin_amdgcn_exp2f(y);
+                s += e;
+                if (kEntropy) sy = __builtin_fmaf(e, y, sy);
+            } else {
+                add<kEntropy>(st, f[k], ref, c);
+            }
+        }
+    }
+    if constexpr (kQuick) {
+        const float off = __builtin_fmaf(-ref, c, -shift);  // below 2^-24 |m c|: 2^off is 1 + off ln 2
+        s = __builtin_fmaf(s * off, kLn2, s);
+        st.s += s;
+        if (kEntropy) st.sy += __builtin_fmaf(s, off, __builtin_fmaf(sy * off, kLn2, sy));
     }
 }
 
+// Whether quick statistics of a row are the row's: its largest logit has put 1 into s, to within rounding, and
+// nothing overflowed.
+template <bool kEntropy>
+__device__ __forceinline__ bool quick_holds(const Stats& st) {
+    return st.s > 0.5f && st.s < INFINITY && (!kEntropy || fabsf(st.sy) < INFINITY);
+}
+
 // The statistics of vectors from + threadIdx.x, + kThreads_, ... below `to`; change(v, n) is applied to vector n.
-template <typename T, bool kEntropy, int kThreads_, typename Change>
+template <typename T, bool kEntropy, bool kQuick, int kThreads_, typename Change>
 __device__ __forceinline__ void read_vecs(Stats& st, const void* vecs, int from, int to, float c, Change change) {
     constexpr int kUnroll = 4;
     const int t = threadIdx.x;
+    vec_t v[kUnroll];
     int n = from;
     for (; n + kUnroll * kThreads_ <= to; n += kUnroll * kThreads_) {
-        vec_t v[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) v[u] = load_vec(vecs, n + u * kThreads_, t);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) change(v[u], n + u * kThreads_ + t);
-        add_vecs<T, kEntropy, kUnroll>(st, v, c);
+        add_vecs<T, kEntropy, kQuick, kUnroll>(st, v, c);
     }
-    for (; n + t < to; n += kThreads_) {
-        vec_t v[1] = {load_vec(vecs, n, t)};
-        change(v[0], n + t);
-        add_vecs<T, kEntropy, 1>(st, v, c);
+    // what is left is on its way all at once, too
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int first = n + u * kThreads_;
+        v[u] = first + t < to ? load_vec(vecs, first, t) : nothing<T>();
     }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+        if (n + u * kThreads_ < to) {
+            const bool in = n + u * kThreads_ + t < to;
+            change(v[u], n + u * kThreads_ + t);
+            if (!kQuick || in) add_vecs<T, kEntropy, kQuick, 1>(st, v + u, c);
+        }
 }
 
 __device__ __forceinline__ float wave_max(float x) {
@@ -380,7 +412,7 @@ struct HeldRow {
     __device__ __forceinline__ Stats stats(float c, Change change) {
         Stats st = no_stats();
         if constexpr (kRest) {
-            read_vecs<T, false, kThreads_>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
+            read_vecs<T, false, false, kThreads_>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
             load_held();
             each([&](vec_t& x, int n) { change(x, n + int(threadIdx.x)); });
         }

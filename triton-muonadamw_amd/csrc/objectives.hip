@@ -18,7 +18,7 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
                                                              float* __restrict__ logprobs,
                                                              float* __restrict__ entropy, float* __restrict__ stats,
                                                              float* __restrict__ coef) {
-    __shared__ Stats lds[kThreads_ / 64];
+    __shared__ Stats lds[2][kThreads_ / 64];
     const uint32_t r = row_of_block();
     if (r >= uint32_t(x.rows)) return;
     const Place at = place(x, r);
@@ -29,13 +29,18 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
         const T* row = row_of<T>(x, at);
         const float xt = chosen(row, token, x.vocab);
         const Span span = span_of(row, x.vocab);
-        Stats st = no_stats();
-        if (int(threadIdx.x) < span.extra) {
-            st.m = widen(row[extra_element<T>(span, threadIdx.x)]);
-            add<kEntropy>(st, st.m, reference(st.m), x.c);
-        }
-        read_vecs<T, kEntropy, kThreads_>(st, row + span.head, 0, span.vecs, x.c, Unchanged());
-        st = over_block<kEntropy, kThreads_>(over_wave<kEntropy>(st, x.c), x.c, lds);
+        auto stats_of_row = [&](auto quick) {
+            constexpr bool kQuick = decltype(quick)::value != 0;
+            Stats st = no_stats();
+            if (int(threadIdx.x) < span.extra) {
+                st.m = widen(row[extra_element<T>(span, threadIdx.x)]);
+                add<kEntropy>(st, st.m, reference(st.m), x.c);
+            }
+            read_vecs<T, kEntropy, kQuick, kThreads_>(st, row + span.head, 0, span.vecs, x.c, Unchanged());
+            return over_block<kEntropy, kThreads_>(over_wave<kEntropy>(st, x.c), x.c, lds[!kQuick]);
+        };
+        Stats st = stats_of_row(Int<1>());
+        if (!quick_holds<kEntropy>(st)) st = stats_of_row(Int<0>());
         const float log_s = logf(st.s);
         lp = (xt - st.m) * x.inv_t - log_s;
         h = log_s - kLn2 * st.sy / st.s;
@@ -271,6 +276,7 @@ int launch_logprobs(const mamw_rows& x, const mamw_per_row& tokens, int64_t igno
         const int64_t vecs = x.vocab / kVec<T>;
         if (vecs <= 512) return go(Int<64>());
         if (vecs <= 2048) return go(Int<256>());
+        if (vecs <= 8192) return go(Int<512>());
         return go(Int<1024>());
     });
 }
