@@ -42,6 +42,7 @@ enum KernelId : int32_t {
     K_OBJ_POLICY,
     K_OBJ_PAIRS,
     K_OBJ_DISTILL,
+    K_OBJ_TEACHER,
     K_COUNT
 };
 

@@ -11,11 +11,13 @@ namespace mamw {
 
 // Rows whose tokens one block of the counting kernel looks at where sequences do not matter.
 constexpr int kCountRows = 1024;
+// Rows of teacher's entries that one workgroup prepares.
+constexpr int kTeacherRows = 16;
 // Bits of the table of a teacher's indices (128 KiB of LDS at most).
 constexpr int64_t kMaxTailVocab = int64_t(1) << 20;
 
-// A workspace: the rows that count of each sequence (or of each kCountRows rows), the length of each row's
-// sequence (policy, by sequence), the rows' parts of the result.
+// A workspace: the rows that count of each sequence (or of each kCountRows or kTeacherRows rows), the length of each
+// row's sequence (policy, by sequence) or its teacher's entries, the rows' parts of the result.
 struct ObjectiveWorkspace {
     int64_t items;      // counts
     size_t lengths_at;  // bytes from the start

@@ -33,6 +33,31 @@ __device__ __forceinline__ bf16_t narrow<bf16_t>(float x) { return {uint16_t(f32
 template <>
 __device__ __forceinline__ _Float16 narrow<_Float16>(float x) { return _Float16(x); }
 
+// An element as it was loaded, in a register of its own: a value that is not looked at yet is not waited for.
+template <typename T>
+struct Raw {
+    uint32_t bits;
+    __device__ __forceinline__ float value() const {
+        if constexpr (sizeof(T) == 4)
+            return __uint_as_float(bits);
+        else if constexpr (__is_same(T, bf16_t))
+            return bf16_to_f32(bits);
+        else
+            return float(__builtin_bit_cast(_Float16, uint16_t(bits)));
+    }
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> raw_at(const T* x) {
+    if constexpr (sizeof(T) == 4)
+        return {*reinterpret_cast<const uint32_t*>(x)};
+    else
+        return {*reinterpret_cast<const uint16_t*>(x)};
+}
+template <typename T>
+__device__ __forceinline__ Raw<T> raw_nothing() {
+    return {sizeof(T) == 4 ? 0xff800000u : __is_same(T, bf16_t) ? 0xff80u : 0xfc00u};
+}
+
 // 16 bytes of a row: kVec<T> elements.
 typedef uint32_t vec_t __attribute__((ext_vector_type(4)));
 typedef vec_t any_vec_t __attribute__((aligned(2)));  // at any element
@@ -367,6 +392,9 @@ __device__ __forceinline__ Stats over_block(const Stats& wave, float c, Stats* l
     return st;
 }
 
+// Loads come back in the order of their issue, and waiting for one is waiting for all before it: what a row needs beside
+// its vectors is loaded before them, so that they are worked on as they arrive.
+//
 // A row in the registers of a workgroup: vector i kThreads + t of the row is v[i] of thread t, single element t its
 // `single`.  Rows longer than that (kRest) have their remaining vectors read twice.
 template <typename T, int kThreads_, int kVecs, bool kRest>
@@ -374,24 +402,35 @@ struct HeldRow {
     const T* row;
     Span span;
     vec_t v[kVecs];
-    float single;
-    float wave_ref;  // float: v holds 2^y below this, once the statistics are taken
+    Raw<T> single_;
+    static constexpr int kGroup = kVecs < 4 ? kVecs : 4, kGroups = kVecs / kGroup;
+    float group_ref[kGroups];  // float: v holds 2^y below its group's, once the statistics are taken
 
     __device__ __forceinline__ const void* vecs() const { return row + span.head; }
 
-    __device__ __forceinline__ void load(const T* row_, int vocab) {
+    __device__ __forceinline__ bool has_single() const { return int(threadIdx.x) < span.extra; }
+    __device__ __forceinline__ float single() const { return has_single() ? single_.value() : -INFINITY; }
+
+    // `spare`: 16 bytes on their boundary that can be read, for rows without a vector.
+    __device__ __forceinline__ void load(const T* row_, int vocab, const void* spare) {
         row = row_;
         span = span_of(row_, vocab);
-        if constexpr (!kRest) load_held();
-        single = int(threadIdx.x) < span.extra ? widen(row_[extra_element<T>(span, threadIdx.x)]) : -INFINITY;
+        single_ = raw_at(row_ + (has_single() ? extra_element<T>(span, threadIdx.x) : 0));
+        if constexpr (!kRest) load_held(spare);
     }
 
-    __device__ __forceinline__ void load_held() {
+    // All kVecs loads whatever the row's length, the last vector again where there is none: with loads that are skipped
+    // the compiler could not count how many are on their way, and would wait for all of them at the first.
+    __device__ __forceinline__ void load_held(const void* spare) {
+        const void* from = span.vecs > 0 ? vecs() : spare;
+        const int last = max(span.vecs - 1, 0);
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int n = i * kThreads_;
-            v[i] = n + int(threadIdx.x) < span.vecs ? load_vec(vecs(), n, threadIdx.x) : nothing<T>();
-        }
+        for (int i = 0; i < kVecs; ++i) v[i] = load_vec(from, 0, min(i * kThreads_ + int(threadIdx.x), last));
+    }
+
+    // Vector i, where it is beyond the row, holds nothing.
+    __device__ __forceinline__ void end_row(int i) {
+        if ((i + 1) * kThreads_ > span.vecs && i * kThreads_ + int(threadIdx.x) >= span.vecs) v[i] = nothing<T>();
     }
 
     // fn(vector, its number less threadIdx.x) for each held one in turn.  The empty statement keeps the compiler from
@@ -413,45 +452,57 @@ struct HeldRow {
         Stats st = no_stats();
         if constexpr (kRest) {
             read_vecs<T, false, false, kThreads_>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
-            load_held();
+            load_held(row);  // never without a vector
             each([&](vec_t& x, int n) { change(x, n + int(threadIdx.x)); });
         }
-        float m = fmaxf(st.m, single);
-        each([&](vec_t& x, int) {
-            float f[kVec<T>];
-            unpack<T>(x, f);
+        // In groups, each as its loads arrive: the sum is taken below the thread's largest logit so far and moved when
+        // that grows, so that only the reductions are left once the last load is there.
+        move_to<false>(st, fmaxf(st.m, single()), c);
+        add<false>(st, single(), reference(st.m), c);
 #pragma unroll
-            for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, f[k]);
-        });
-        move_to<false>(st, wave_max(m), c);
-        const float ref = wave_ref = reference(st.m);
-        add<false>(st, single, ref, c);
-        each([&](vec_t& x, int) {
-            float f[kVec<T>];
-            unpack<T>(x, f);
+        for (int q = 0; q < kGroups; ++q)
+            if (q * kGroup * kThreads_ < span.vecs) {
+                float m = st.m;
 #pragma unroll
-            for (int k = 0; k < kVec<T>; ++k) {
-                f[k] = __builtin_amdgcn_exp2f(below(f[k], ref, c));
-                st.s += f[k];
+                for (int i = q * kGroup; i < (q + 1) * kGroup; ++i) {
+                    end_row(i);
+                    float f[kVec<T>];
+                    unpack<T>(v[i], f);
+#pragma unroll
+                    for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, f[k]);
+                }
+                move_to<false>(st, m, c);
+                const float ref = group_ref[q] = reference(m);
+#pragma unroll
+                for (int i = q * kGroup; i < (q + 1) * kGroup; ++i) {
+                    asm volatile("" : "+v"(v[i]));
+                    float f[kVec<T>];
+                    unpack<T>(v[i], f);
+#pragma unroll
+                    for (int k = 0; k < kVec<T>; ++k) {
+                        f[k] = __builtin_amdgcn_exp2f(below(f[k], ref, c));
+                        st.s += f[k];
+                    }
+                    if constexpr (sizeof(T) == 4) v[i] = pack<T>(f);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // the next group is not begun, and waited for, before
             }
-            if constexpr (sizeof(T) == 4) x = pack<T>(f);
-        });
-        st.s = wave_sum(st.s);
-        return st;
+        return over_wave<false>(st, c);
     }
 
     // g_j = b 2^y below m.
     template <typename Change>
     __device__ __forceinline__ void write(T* __restrict__ g, float b, float m, float c, Change change) {
-        const float from_wave = b * __builtin_amdgcn_exp2f(below(wave_ref, m, c));
         T* at = g + span.head;
         const int t = threadIdx.x;
         each([&](vec_t& x, int n) {
             float f[kVec<T>];
             unpack<T>(x, f);
+            const float group =
+                sizeof(T) == 4 ? b * __builtin_amdgcn_exp2f(below(group_ref[n / kThreads_ / kGroup], m, c)) : b;
 #pragma unroll
             for (int k = 0; k < kVec<T>; ++k)
-                f[k] = sizeof(T) == 4 ? from_wave * f[k] : b * __builtin_amdgcn_exp2f(below(f[k], m, c));
+                f[k] = group * (sizeof(T) == 4 ? f[k] : __builtin_amdgcn_exp2f(below(f[k], m, c)));
             if (n + t < span.vecs) store_vec(at, n, t, pack<T>(f));
         });
         if constexpr (kRest) {
@@ -475,8 +526,8 @@ struct HeldRow {
                 }
             }
         }
-        if (t < span.extra)
-            g[extra_element<T>(span, threadIdx.x)] = narrow<T>(b * __builtin_amdgcn_exp2f(below(single, m, c)));
+        if (has_single())
+            g[extra_element<T>(span, threadIdx.x)] = narrow<T>(b * __builtin_amdgcn_exp2f(below(single(), m, c)));
     }
 };
 
@@ -484,12 +535,25 @@ struct Unchanged {
     __device__ __forceinline__ void operator()(vec_t&, int) const {}
 };
 
-// The number that weights are divided by: rows that count, or sequences that have any.  Every wave by itself.
-__device__ __forceinline__ float count_all(const int32_t* __restrict__ count, int64_t items, bool by_sequence) {
-    float n = 0.f;
-    for (int64_t i = threadIdx.x % 64; i < items; i += 64) n += by_sequence ? float(count[i] > 0) : float(count[i]);
-    return fmaxf(wave_sum(n), 1.f);
-}
+// The number that weights are divided by: rows that count, or sequences that have any.  Every wave by itself; the load
+// of the first 64 counts is apart, to be on its way before a row's.
+struct Counts {
+    const int32_t* count;
+    int64_t items;  // at least 1
+    bool by_sequence;
+    int32_t first;
+
+    __device__ __forceinline__ Counts(const int32_t* count_, int64_t items_, bool by_sequence_)
+        : count(count_), items(items_), by_sequence(by_sequence_),
+          first(count_[min(int64_t(threadIdx.x % 64), items_ - 1)]) {}
+    __device__ __forceinline__ float one(int32_t n) const { return by_sequence ? float(n > 0) : float(n); }
+    __device__ __forceinline__ float all() const {
+        const int lane = threadIdx.x % 64;
+        float n = lane < items ? one(first) : 0.f;
+        for (int64_t i = 64 + lane; i < items; i += 64) n += one(count[i]);
+        return fmaxf(wave_sum(n), 1.f);
+    }
+};
 
 // ---- launches
 
@@ -531,7 +595,7 @@ inline double row_bytes(const mamw_rows& x, bool grad) {
 
 // fn(workgroup size, vectors a thread, whether some are left) for rows of `vecs` vectors, held by one workgroup.
 // Each thread keeps one to sixteen: fewer threads of more would leave the reductions to fewer waves, and a row of 256
-// KiB is all the registers of a compute unit that its other values leave.  A longer row keeps 224 KiB and has the rest
+// KiB is all the registers of a compute unit that its other values leave.  A longer row keeps 192 KiB and has the rest
 // read twice.
 template <int kN>
 struct Int {
@@ -546,7 +610,7 @@ int with_held_row(int64_t vecs, Fn fn) {
     if (vecs <= 4096) return fn(Int<512>(), Int<8>(), Int<0>());
     if (vecs <= 8192) return fn(Int<512>(), Int<16>(), Int<0>());
     if (vecs <= 16384) return fn(Int<1024>(), Int<16>(), Int<0>());
-    return fn(Int<1024>(), Int<14>(), Int<1>());
+    return fn(Int<1024>(), Int<12>(), Int<1>());
 }
 
 // One workgroup a row.  Such workgroups come and go by themselves: a row's loads do not wait for the stores of the row

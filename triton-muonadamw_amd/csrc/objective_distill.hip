@@ -1,17 +1,15 @@
-// Distillation from a teacher's top logits for gfx950: the divergence of a row and its gradient in one pass.
+// Distillation from a teacher's top logits for gfx950: the teacher's entries of all rows first, then the divergence of
+// a row and its gradient in one pass.
 #include "mamw_rows.h"
 
 namespace mamw {
 namespace {
 
-// ---- distillation
+// ---- the teacher's entries
 
-struct Distill {
+struct TeacherArgs {
     PerRow logits, indices, lse, mask;
-    int64_t items;
     int k;
-    float temperature, scale;
-    const int32_t* count;
 };
 
 __device__ __forceinline__ float load_float(const PerRow& a, int64_t i) {
@@ -20,37 +18,192 @@ __device__ __forceinline__ float load_float(const PerRow& a, int64_t i) {
     return widen(reinterpret_cast<const _Float16*>(a.data)[i]);
 }
 
-// The teacher's part of a row, by one wave; the others have it after the next barrier.
-struct Teacher {
-    float sum_p;   // of all entries
-    float x_top;   // the student's largest logit among them
-    int entries;   // different ones
-    int repeated;  // some are given more than once
-    int beyond;    // some are outside the vocabulary
+constexpr int kPadding = -1;
+
+// What the student's pass needs of a row's teacher: for each entry its index (kPadding: left out) and probability, and
+struct TeacherRow {
+    float sum_p, plogp;  // sum of p and of p log p
+    int entries;         // different ones
+    int beyond;          // some are outside the vocabulary
+};
+static_assert(sizeof(TeacherRow) == 16, "one 16-byte load a row");
+
+// One wave a row, kTeacherRows rows a workgroup; entry k of the row is entry k / 64 of lane k % 64.  By itself, in
+// front of the student's pass: there it would be one wave's chain of dependent steps while fifteen wait for it, once
+// a row (128 entries: 16 us of 181 for 2048 rows of 128256 bf16).
+//
+// An index that is given more than once becomes one entry with the sum of the probabilities.  A table of 2^14 bits
+// finds those that may be: an entry whose bit is set already, by its own index or by another that falls on it, is
+// compared with all others.
+constexpr int kSeenBits = 1 << 14;
+
+template <int kPerLane, bool kTail>
+__global__ __launch_bounds__(64 * kTeacherRows) void teacher_kernel(Rows x, TeacherArgs a, int32_t* __restrict__ index,
+                                                                    float* __restrict__ probs,
+                                                                    TeacherRow* __restrict__ info, uint32_t items,
+                                                                    int32_t* __restrict__ count) {
+    __shared__ uint32_t seen_bits[kTeacherRows][kSeenBits / 32];
+    __shared__ int active[kTeacherRows];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const uint32_t item = row_of_block();
+    if (item >= items) return;
+    const int64_t r = int64_t(item) * kTeacherRows + __builtin_amdgcn_readfirstlane(wave);
+    bool counts_ = false;
+    if (r < x.rows) {
+        const Place at = place(x, uint32_t(r));
+        counts_ = load_mask(a.mask, at);
+        if (counts_) {
+            uint32_t* seen = seen_bits[wave];
+#pragma unroll
+            for (int i = 0; i < kSeenBits / 32 / 64; ++i) seen[i * 64 + lane] = 0;
+            const int64_t tl = offset(a.logits, at), ti = offset(a.indices, at);
+            int32_t idx[kPerLane];
+            float t[kPerLane];
+            bool beyond = false;
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) {
+                const int k = e * 64 + lane;
+                const bool is = k < a.k;
+                t[e] = is ? load_float(a.logits, tl + k) : -INFINITY;
+                const int64_t j = is ? load_int(a.indices, ti + k) : -1;
+                beyond |= j >= x.vocab;
+                const bool in = j >= 0 && j < x.vocab && t[e] != -INFINITY;
+                idx[e] = in ? int32_t(j) : kPadding;
+                if (in) top = fmaxf(top, t[e]);
+            }
+            float shift;
+            if constexpr (kTail) {
+                top = 0.f;
+                shift = load_f32(a.lse, at);
+            } else {
+                top = wave_max(top);
+                float z = 0.f;
+#pragma unroll
+                for (int e = 0; e < kPerLane; ++e)
+                    if (idx[e] >= 0) z += __builtin_amdgcn_exp2f(below(t[e], top, x.c));
+                shift = logf(wave_sum(z));
+            }
+            float sum_p = 0.f, plogp = 0.f;
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) {
+                if (idx[e] < 0) continue;
+                const float l = (t[e] - top) * x.inv_t - shift, p = expf(l);
+                sum_p += p;
+                plogp += p > 0.f ? p * l : p;  // p log p = 0 at p = 0; NaN stays
+                t[e] = p;
+            }
+            sum_p = wave_sum(sum_p);
+            plogp = wave_sum(plogp);
+            // the bits of one wave are its own: its LDS accesses stay in order
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            uint64_t again[kPerLane];
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) {
+                const uint32_t h = uint32_t(idx[e]) % kSeenBits, bit = 1u << (h & 31);
+                again[e] = __ballot(idx[e] >= 0 && (atomicOr(&seen[h >> 5], bit) & bit));
+            }
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e)
+                while (again[e]) {
+                    const int l = __builtin_ctzll(again[e]);
+                    again[e] &= again[e] - 1;
+                    const int j = __builtin_amdgcn_readlane(idx[e], l);
+                    if (j < 0) continue;  // made one with an earlier entry meanwhile
+                    float p = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kPerLane; ++i) p += idx[i] == j ? t[i] : 0.f;
+                    p = wave_sum(p);
+                    bool found = false;
+#pragma unroll
+                    for (int i = 0; i < kPerLane; ++i) {
+                        const uint64_t same = __ballot(idx[i] == j);
+                        if (idx[i] == j) {
+                            const bool first = !found && lane == __builtin_ctzll(same);
+                            t[i] = p;
+                            idx[i] = first ? j : kPadding;
+                        }
+                        found |= same != 0;
+                    }
+                }
+            int entries = 0;
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) {
+                const int k = e * 64 + lane;
+                entries += __popcll(__ballot(idx[e] >= 0));
+                if (k < a.k) {
+                    index[r * a.k + k] = idx[e];
+                    probs[r * a.k + k] = t[e];
+                }
+            }
+            const bool any_beyond = __any(beyond);
+            if (lane == 0) info[r] = {sum_p, plogp, entries, any_beyond};
+        }
+    }
+    if (lane == 0) active[wave] = counts_;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int n = 0;
+        for (int w = 0; w < kTeacherRows; ++w) n += active[w];
+        count[item] = n;
+    }
+}
+
+// ---- the student's rows
+
+struct Distill {
+    PerRow mask;
+    int64_t items;
+    int k;
+    float temperature, scale;
+    const int32_t* count;
+    const int32_t* index;
+    const float* probs;
+    const TeacherRow* info;
 };
 
-// An entry of LDS: its index, or kPadding, or kRepeated - its index where an entry before it has the same.
-constexpr int kPadding = -1, kRepeated = -2;
+// A wave's part of a row: its statistics, of the teacher's entries alone the sum s_in of 2^y, the sum p of their
+// probabilities and px of p (x - m).
+struct Parts {
+    float m, s, s_in, p, px;
+};
 
-// kTail: the teacher's entries are taken out of the row (an index in `marked`, a bit for each entry of the
-// vocabulary) and their sum is added from the gathered logits, so that the sum over all others is not the small
-// difference of two large ones.  The same bits find repeated entries; where the vocabulary is too large for them
-// (bits = 0, never with kTail) every pair of entries is compared.
+template <int kThreads_>
+__device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* lds) {
+    constexpr int kN = kThreads_ / 64;
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = mine;
+    __syncthreads();
+    mine = lds[threadIdx.x % kN];
+    float m = mine.m;
+#pragma unroll
+    for (int o = kN / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float f = __builtin_amdgcn_exp2f(fmaxf(below(mine.m, reference(m), c), -1e30f));
+    mine.s *= f;
+    mine.s_in *= f;
+    mine.px += mine.p * (reference(mine.m) - reference(m));
+#pragma unroll
+    for (int o = kN / 2; o >= 1; o >>= 1) {
+        mine.s += __shfl_xor(mine.s, o, 64);
+        mine.s_in += __shfl_xor(mine.s_in, o, 64);
+        mine.p += __shfl_xor(mine.p, o, 64);
+        mine.px += __shfl_xor(mine.px, o, 64);
+    }
+    mine.m = m;
+    return mine;
+}
+
+// kTail: the teacher's entries are taken out of the row (marked in a table of a bit for each entry of the vocabulary)
+// and their sum is added from the gathered logits, so that the sum over all others is not the small difference of two
+// large ones.
 template <typename T, int kThreads_, int kVecs, bool kRest, bool kTail>
 __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
     Rows x, Distill p, int bits, float4* __restrict__ partials, const float* __restrict__ scale, int unless_one,
     T* __restrict__ grad) {
-    extern __shared__ uint32_t dynamic[];
-    __shared__ Stats lds[kThreads_ / 64];
-    __shared__ Teacher teacher;
-    uint32_t* marked = dynamic;
-    int32_t* index = reinterpret_cast<int32_t*>(marked + bits);
-    float* logp = reinterpret_cast<float*>(index + p.k);
-    float* xs = logp + p.k;
+    extern __shared__ uint32_t marked[];
+    __shared__ Parts lds[kThreads_ / 64];
+    constexpr int kEntries = MAMW_MAX_TEACHER / kThreads_;  // of a thread
     const float f = scale ? *scale : 1.f;
     if (scale && unless_one && f == 1.f) return;
-    for (int j = threadIdx.x; j < bits; j += kThreads_) marked[j] = 0;
-    const int lane = threadIdx.x;
     const uint32_t r = row_of_block();
     if (r >= uint32_t(x.rows)) return;
     const Place at = place(x, r);
@@ -61,47 +214,40 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
         return;
     }
     const T* row = row_of<T>(x, at);
-    HeldRow<T, kThreads_, kVecs, kRest> held;
-    held.load(row, x.vocab);
-    const float all = count_all(p.count, p.items, false);
-    __syncthreads();  // the bits are clear
-    if (threadIdx.x < 64) {
-        const int64_t tl = offset(p.logits, at), ti = offset(p.indices, at);
-        bool beyond = false, repeated = bits == 0;
-#pragma unroll 1
-        for (int k = lane; k < p.k; k += 64) {
-            const float t = load_float(p.logits, tl + k);
-            const int64_t j = load_int(p.indices, ti + k);
-            const bool in = j >= 0 && j < x.vocab && t != -INFINITY;
-            beyond |= j >= x.vocab;
-            index[k] = in ? int32_t(j) : kPadding;
-            logp[k] = t;
-            xs[k] = in ? widen(row[j]) : -INFINITY;
-            if (in && bits) repeated |= (atomicOr(&marked[j >> 5], 1u << (j & 31)) >> (j & 31)) & 1u;
-        }
-        if (__any(repeated)) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-            for (int k = lane; k < p.k; k += 64) {
-                int before = 0;
-                const int j = index[k];
-                for (int i = 0; i < k; ++i) before += index[i] == j || index[i] == kRepeated - j;
-                if (j >= 0 && before) index[k] = kRepeated - j;
-            }
-        }
-        const int any_repeated = __any(repeated), any_beyond = __any(beyond);
-        if (lane == 0) {
-            teacher.repeated = any_repeated;
-            teacher.beyond = any_beyond;
+    // The entries' indices before the row, to mark them while it is on its way; the logits they point to behind it, to be
+    // looked at where it has been waited for anyway.
+    int32_t index[kEntries];
+    float probs[kEntries];
+    Raw<T> xs[kEntries];
+#pragma unroll
+    for (int e = 0; e < kEntries; ++e) {
+        const int k = e * kThreads_ + int(threadIdx.x);
+        index[e] = kPadding;
+        probs[e] = 0.f;
+        if (k < p.k) {
+            index[e] = p.index[int64_t(r) * p.k + k];
+            probs[e] = p.probs[int64_t(r) * p.k + k];
         }
     }
+    const TeacherRow teacher = p.info[r];
+    const Counts counted(p.count, p.items, false);
+    HeldRow<T, kThreads_, kVecs, kRest> held;
+    held.load(row, x.vocab, p.count);
+    if constexpr (kTail) {
+        for (int j = threadIdx.x; j < bits; j += kThreads_) marked[j] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEntries; ++e)
+            if (index[e] >= 0) atomicOr(&marked[index[e] >> 5], 1u << (index[e] & 31));
+    }
+#pragma unroll
+    for (int e = 0; e < kEntries; ++e) xs[e] = raw_at(row + max(index[e], 0));
     auto take_out = [&](vec_t& v, int n) {
         if constexpr (kTail) {
             // the bits of vector n: elements head + n kVec and on
             const int j = held.span.head + n * kVec<T>;
             const uint32_t w = j >> 5;
-            if (n >= held.span.vecs) return;
+            if (n >= held.span.vecs) return;  // (the copies of the last vector become nothing later)
             uint32_t m = marked[w] >> (j & 31);
             if ((j & 31) + kVec<T> > 32 && int(w) + 1 < bits) m |= marked[w + 1] << (32 - (j & 31));
             m &= (1u << kVec<T>) - 1u;
@@ -127,119 +273,110 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
                 if (n / kThreads_ % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             });
         const int j = extra_element<T>(held.span, threadIdx.x);
-        if (int(threadIdx.x) < held.span.extra && (marked[j >> 5] >> (j & 31) & 1u)) held.single = -INFINITY;
+        if (int(threadIdx.x) < held.span.extra && (marked[j >> 5] >> (j & 31) & 1u))
+            held.single_ = raw_nothing<T>();
     }
-    if (threadIdx.x < 64) {
-        float shift = 0.f, top = 0.f;
-        if constexpr (kTail) {
-            shift = load_f32(p.lse, at);
-        } else {
-            top = -INFINITY;
-#pragma unroll 1
-            for (int k = lane; k < p.k; k += 64) top = index[k] != kPadding ? fmaxf(top, logp[k]) : top;
-            top = wave_max(top);
-            float z = 0.f;
-#pragma unroll 1
-            for (int k = lane; k < p.k; k += 64)
-                if (index[k] != kPadding) z += __builtin_amdgcn_exp2f(below(logp[k], top, x.c));
-            shift = logf(wave_sum(z));
-        }
-        float sum_p = 0.f, x_top = -INFINITY;
-        int entries = 0;
-#pragma unroll 1
-        for (int k = lane; k < p.k; k += 64) {
-            if (index[k] == kPadding) continue;
-            const float l = (logp[k] - top) * x.inv_t - shift;
-            logp[k] = l;
-            sum_p += expf(l);
-            x_top = fmaxf(x_top, xs[k]);
-            entries += index[k] >= 0;
-        }
-        sum_p = wave_sum(sum_p);
-        x_top = wave_max(x_top);
+    Stats wave = held.stats(x.c, take_out);
+    if constexpr (kTail) {
+        float x_top = -INFINITY;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) entries += __shfl_xor(entries, o, 64);
-        if (lane == 0) {
-            teacher.sum_p = sum_p;
-            teacher.x_top = x_top;
-            teacher.entries = entries;
-        }
+        for (int e = 0; e < kEntries; ++e)
+            if (index[e] >= 0) x_top = fmaxf(x_top, xs[e].value());
+        move_to<false>(wave, fmaxf(wave.m, wave_max(x_top)), x.c);
     }
-    const Stats wave = held.stats(x.c, take_out);
-    Stats st;
-    if constexpr (kTail) {
-        // x_top is wave 0's: it reaches the reference through the waves' statistics
-        Stats mine = wave;
-        if (threadIdx.x < 64) move_to<false>(mine, fmaxf(wave.m, wave_max(lane == 0 ? teacher.x_top : -INFINITY)), x.c);
-        st = over_block<false, kThreads_>(mine, x.c, lds);
-    } else {
-        st = over_block<false, kThreads_>(wave, x.c, lds);
+    const float ref = reference(wave.m);
+    float s_in = 0.f, sum_p = 0.f, px = 0.f;
+#pragma unroll
+    for (int e = 0; e < kEntries; ++e) {
+        if (index[e] < 0) continue;
+        if (kTail) s_in += __builtin_amdgcn_exp2f(below(xs[e].value(), ref, x.c));
+        sum_p += probs[e];
+        px += probs[e] > 0.f ? probs[e] * (xs[e].value() - ref) : probs[e];  // 0 * -inf; NaN stays
     }
-    const float s_out = st.s;
-    if constexpr (kTail) {
-        float s_in = 0.f;
-#pragma unroll 1
-        for (int k = threadIdx.x % 64; k < p.k; k += 64)
-            if (index[k] >= 0) s_in += __builtin_amdgcn_exp2f(below(xs[k], st.m, x.c));
-        st.s += wave_sum(s_in);
-    }
-    const bool beyond = teacher.beyond;
+    const Parts all_parts = parts_over_block<kThreads_>(
+        {wave.m, wave.s, wave_sum(s_in), wave_sum(sum_p), wave_sum(px)}, x.c, lds);
+    const float m = all_parts.m, s = all_parts.s + all_parts.s_in, inv_s = 1.f / s;
+    const float count = counted.all();
+    // sum p (log p - log q), with log q = (x - m) / T - log s
+    float loss = teacher.plogp - all_parts.px * x.inv_t + teacher.sum_p * logf(s);
     float share = teacher.entries > 0 ? 1.f : 0.f;  // of q_j outside the teacher's entries
     const float in = kTail ? 1.f : share;
-    float rest_loss = 0.f;
+    if (teacher.entries == 0) loss = 0.f;
     if constexpr (kTail) {
         share = 1.f;
         if (teacher.entries < x.vocab) {
-            const float rest_q = s_out / st.s, rest_p = fmaxf(1.f - teacher.sum_p, kSmallestTail);
-            rest_loss = rest_p * logf(rest_p / rest_q);
+            const float rest_q = all_parts.s / s, rest_p = fmaxf(1.f - teacher.sum_p, kSmallestTail);
+            loss += rest_p * logf(rest_p / rest_q);
             share = 1.f - rest_p / rest_q;
         }
     }
-    if (threadIdx.x < 64 && partials) {
-        const float log_s = logf(st.s);
-        float loss = 0.f;
-#pragma unroll 1
-        for (int k = lane; k < p.k; k += 64) {
-            if (index[k] == kPadding) continue;
-            const float prob = expf(logp[k]);
-            // p log p = 0 at p = 0; NaN stays
-            loss += prob > 0.f ? prob * (logp[k] - ((xs[k] - st.m) * x.inv_t - log_s)) : prob;
-        }
-        loss = wave_sum(loss) + rest_loss;
-        if (lane == 0) partials[r] = make_float4((beyond ? NAN : loss) / all, 0.f, 0.f, 0.f);
-    }
+    if (partials && threadIdx.x == 0)
+        partials[r] = make_float4((teacher.beyond ? NAN : loss) / count, 0.f, 0.f, 0.f);
     if (g) {
-        const float w = beyond ? NAN : f * p.scale * p.temperature / all, inv_s = 1.f / st.s;
-        held.write(g, w * share * inv_s, st.m, x.c, take_out);
+        const float w = teacher.beyond ? NAN : f * p.scale * p.temperature / count;
+        held.write(g, w * share * inv_s, m, x.c, take_out);
         __syncthreads();  // then the entries themselves, over what was written there
-        for (int k = threadIdx.x; k < p.k; k += kThreads_) {
-            const int j = index[k];
-            if (j < 0) continue;
-            float prob = expf(logp[k]);
-            if (teacher.repeated)
-                for (int i = k + 1; i < p.k; ++i) prob += index[i] == kRepeated - j ? expf(logp[i]) : 0.f;
-            g[j] = narrow<T>(w * (in * inv_s * __builtin_amdgcn_exp2f(below(xs[k], st.m, x.c)) - prob));
-        }
+#pragma unroll
+        for (int e = 0; e < kEntries; ++e)
+            if (index[e] >= 0)
+                g[index[e]] = narrow<T>(w * (in * inv_s * __builtin_amdgcn_exp2f(below(xs[e].value(), m, x.c)) - probs[e]));
     }
 }
 
-int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWorkspace& ws, float4* partials,
-                   const float* scale, int unless_one, void* grad, char* base, hipStream_t stream) {
+// ---- launches
+
+struct DistillWorkspace {
+    int32_t* count;
+    int32_t* index;
+    float* probs;
+    float4* partials;
+    TeacherRow* info;
+};
+
+DistillWorkspace parts_of(const ObjectiveWorkspace& ws, char* base, int64_t rows, int64_t k) {
+    DistillWorkspace w;
+    w.count = reinterpret_cast<int32_t*>(base);
+    w.index = reinterpret_cast<int32_t*>(base + ws.lengths_at);
+    w.probs = reinterpret_cast<float*>(w.index + rows * k);
+    w.partials = reinterpret_cast<float4*>(base + ws.partials_at);
+    w.info = reinterpret_cast<TeacherRow*>(w.partials + rows);
+    return w;
+}
+
+int launch_teacher(const mamw_rows& x, const mamw_distill& p, const ObjectiveWorkspace& ws, const DistillWorkspace& w,
+                   hipStream_t stream) {
+    const Rows rows = make_rows(x, p.temperature);
+    if (rows.rows == 0) return MAMW_OK;
+    const TeacherArgs a = {make_per_row(p.teacher_logits), make_per_row(p.teacher_indices),
+                           make_per_row(p.teacher_lse), make_per_row(p.mask), int(p.k)};
+    auto go = [&](auto n) {
+        constexpr int kPerLane = decltype(n)::value;
+        return int(launch(K_OBJ_TEACHER, kPerLane, 0.0, 0.0,
+                          p.teacher_lse.data ? teacher_kernel<kPerLane, true> : teacher_kernel<kPerLane, false>,
+                          row_grid(ws.items), dim3(64 * kTeacherRows), stream, rows, a, w.index, w.probs, w.info,
+                          uint32_t(ws.items), w.count));
+    };
+    return p.k <= 64 ? go(Int<1>()) : p.k <= 128 ? go(Int<2>()) : p.k <= 256 ? go(Int<4>())
+         : p.k <= 512 ? go(Int<8>()) : go(Int<16>());
+}
+
+int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWorkspace& ws, const DistillWorkspace& w,
+                   float4* partials, const float* scale, int unless_one, void* grad, hipStream_t stream) {
     const Rows rows = make_rows(x, p.temperature);
     if (rows.rows == 0) return MAMW_OK;
     Distill d;
-    d.logits = make_per_row(p.teacher_logits);
-    d.indices = make_per_row(p.teacher_indices);
-    d.lse = make_per_row(p.teacher_lse);
     d.mask = make_per_row(p.mask);
     d.items = ws.items;
     d.k = int(p.k);
     d.temperature = p.temperature;
     d.scale = p.scale;
-    d.count = reinterpret_cast<const int32_t*>(base);
+    d.count = w.count;
+    d.index = w.index;
+    d.probs = w.probs;
+    d.info = w.info;
     const bool tail = p.teacher_lse.data != nullptr;
-    const int bits = x.vocab <= kMaxTailVocab ? int((x.vocab + 31) / 32) : 0;
-    const size_t lds = size_t(bits) * 4 + size_t(d.k) * 12;
+    const int bits = tail ? int((x.vocab + 31) / 32) : 0;
+    const size_t lds = size_t(bits) * 4;
     return with_type(x.type, [&](auto t) {
         using T = decltype(t);
         return with_held_row(x.vocab / kVec<T>, [&](auto n, auto v, auto rest) {
@@ -247,8 +384,8 @@ int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWor
             constexpr bool kRest = decltype(rest)::value != 0;
             return int(launch_lds(K_OBJ_DISTILL, kN + tail, 0.0, row_bytes(x, grad != nullptr),
                                   tail ? distill_kernel<T, kN, kV, kRest, true> : distill_kernel<T, kN, kV, kRest, false>,
-                                  row_grid(rows.rows), dim3(kN), lds, stream, rows, d, bits,
-                                  partials, scale, unless_one, static_cast<T*>(grad)));
+                                  row_grid(rows.rows), dim3(kN), lds, stream, rows, d, bits, partials, scale,
+                                  unless_one, static_cast<T*>(grad)));
         });
     });
 }
@@ -273,15 +410,13 @@ extern "C" int mamw_distill_loss(const mamw_rows* logits, const mamw_distill* p,
     if (st != MAMW_OK) return st;
     if ((st = check_workspace(ws, workspace, workspace_bytes)) != MAMW_OK) return st;
     if (!result) return MAMW_ERR_NULL;
-    const Rows rows = make_rows(*logits, p->temperature);
+    const int64_t rows = logits->outer * logits->inner;
     char* base = static_cast<char*>(workspace);
-    float4* partials = reinterpret_cast<float4*>(base + ws.partials_at);
+    const DistillWorkspace w = parts_of(ws, base, rows, p->k);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const PerRow none = {};
-    if ((st = launch_count(rows, none, 0, make_per_row(p->mask), {nullptr, 0}, ws, false, base, s)) != MAMW_OK)
-        return st;
-    if ((st = launch_distill(*logits, *p, ws, partials, nullptr, 0, grad, base, s)) != MAMW_OK) return st;
-    return launch_result(ws, base, rows.rows, p->scale * p->temperature * p->temperature, result, s);
+    if ((st = launch_teacher(*logits, *p, ws, w, s)) != MAMW_OK) return st;
+    if ((st = launch_distill(*logits, *p, ws, w, w.partials, nullptr, 0, grad, s)) != MAMW_OK) return st;
+    return launch_result(ws, base, rows, p->scale * p->temperature * p->temperature, result, s);
 }
 
 extern "C" int mamw_distill_grad(const mamw_rows* logits, const mamw_distill* p, const float* scale, int unless_one,
@@ -290,7 +425,8 @@ extern "C" int mamw_distill_grad(const mamw_rows* logits, const mamw_distill* p,
     int st = check_distill(logits, p, grad, &ws);
     if (st != MAMW_OK) return st;
     if ((st = check_workspace(ws, workspace, workspace_bytes)) != MAMW_OK) return st;
-    if (!scale || (!grad && logits->outer * logits->inner > 0)) return MAMW_ERR_NULL;
-    return launch_distill(*logits, *p, ws, nullptr, scale, unless_one, grad, static_cast<char*>(workspace),
-                          static_cast<hipStream_t>(stream));
+    const int64_t rows = logits->outer * logits->inner;
+    if (!scale || (!grad && rows > 0)) return MAMW_ERR_NULL;
+    const DistillWorkspace w = parts_of(ws, static_cast<char*>(workspace), rows, p->k);
+    return launch_distill(*logits, *p, ws, w, nullptr, scale, unless_one, grad, static_cast<hipStream_t>(stream));
 }

@@ -34,13 +34,18 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
         if (g) zero_row(g, x.vocab, kThreads_);
         return;
     }
-    HeldRow<T, kThreads_, kVecs, kRest> held;
-    held.load(row_of<T>(x, at), x.vocab);
-    const float xt = chosen(held.row, token, x.vocab);
-    const float w = 1.f / (length * count_all(p.count, p.items, p.by_sequence));
+    const T* row = row_of<T>(x, at);
+    const bool beyond = token < 0 || token >= x.vocab;
+    const Raw<T> xt_ = raw_at(row + (beyond ? 0 : token));
+    const Counts counted(p.count, p.items, p.by_sequence);
     const float old = load_f32(p.old, at), adv = load_f32(p.advantages, at);
+    const float ref = p.ref.data ? load_f32(p.ref, at) : 0.f;
+    HeldRow<T, kThreads_, kVecs, kRest> held;
+    held.load(row, x.vocab, p.count);
     const Stats wave = held.stats(x.c, Unchanged());
     const Stats st = over_block<false, kThreads_>(wave, x.c, lds);
+    const float w = 1.f / (length * counted.all());
+    const float xt = beyond ? NAN : xt_.value();
     const float lp = (xt - st.m) * x.inv_t - logf(st.s);
     const float ratio = expf(lp - old);
     const float bound = fminf(fmaxf(ratio, 1.f - p.low), 1.f + p.high);
@@ -48,7 +53,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
     float loss = -(clipped ? bound : ratio) * adv, kl = 0.f;
     float slope = clipped ? 0.f : -adv * ratio;
     if (p.ref.data) {
-        const float d = load_f32(p.ref, at) - lp, e = expm1f(d);
+        const float d = ref - lp, e = expm1f(d);
         kl = e - d;
         loss += p.kl_coef * kl;
         slope -= p.kl_coef * e;
@@ -58,7 +63,6 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
         if (partials) partials[r] = make_float4(w * p.scale * loss, w * kl, clipped ? w : 0.f, 0.f);
     }
     if (g) {
-        const bool beyond = token < 0 || token >= x.vocab;
         const float a = beyond ? NAN : f * p.scale * w * slope * x.inv_t, b = -a / st.s;
         held.write(g, b, st.m, x.c, Unchanged());
         // by the thread that wrote the element: its writes stay in order

@@ -146,16 +146,18 @@ __device__ __forceinline__ bool counts(const Rows& x, const PerRow& tokens, int6
 // counts[i]: rows that count of sequence i, and in lengths[] for each row of the sequence; or, with no sequences
 // (lengths NULL), of the kCountRows rows from i kCountRows on.
 __global__ __launch_bounds__(kThreads) void count_kernel(Rows x, PerRow tokens, int64_t ignore, PerRow mask,
-                                                         Sequences seqs, int32_t* __restrict__ count,
+                                                         Sequences seqs, uint32_t items, int32_t* __restrict__ count,
                                                          float* __restrict__ lengths) {
     __shared__ float lds[kWaves];
-    int64_t from = int64_t(blockIdx.x) * kCountRows, to = min(from + kCountRows, int64_t(x.rows));
-    if (lengths) sequence_rows(seqs, x, blockIdx.x, &from, &to);
+    const uint32_t item = row_of_block();
+    if (item >= items) return;
+    int64_t from = int64_t(item) * kCountRows, to = min(from + kCountRows, int64_t(x.rows));
+    if (lengths) sequence_rows(seqs, x, item, &from, &to);
     int n = 0;
     for (int64_t r = from + threadIdx.x; r < to; r += kThreads) n += counts(x, tokens, ignore, mask, uint32_t(r));
     // below 2^24 a thread; exact as floats where the sum is, too, else the weight's last bit
     const float all = block_sum(Floats<1>{{float(n)}}, lds).v[0];
-    if (threadIdx.x == 0) count[blockIdx.x] = int32_t(all);
+    if (threadIdx.x == 0) count[item] = int32_t(all);
     if (lengths)
         for (int64_t r = from + threadIdx.x; r < to; r += kThreads) lengths[r] = all;
 }
@@ -201,7 +203,8 @@ __global__ __launch_bounds__(kThreads) void pairs_kernel(Rows x, Preference p, c
                                                          float* __restrict__ logprobs, float* __restrict__ rewards,
                                                          float* __restrict__ losses, float* __restrict__ coef) {
     __shared__ float lds[kWaves * 2];
-    const int64_t pairs = p.seqs.count / 2, i = blockIdx.x;
+    const int64_t pairs = p.seqs.count / 2, i = row_of_block();
+    if (i >= pairs) return;
     const PerRow none = {};
     int64_t from[2], to[2];
     // Sums of a thousand log-probabilities, whose differences to a reference's are what counts: in 64 bits, as is a
@@ -292,8 +295,8 @@ int launch_count(const Rows& rows, const PerRow& tokens, int64_t ignore, const P
         if (st != 0) return st;
     }
     if (ws.items == 0) return MAMW_OK;
-    return int(launch(K_OBJ_COUNT, 0, 0.0, 0.0, count_kernel, dim3(unsigned(ws.items)), dim3(kThreads), stream, rows,
-                      tokens, ignore, mask, seqs, reinterpret_cast<int32_t*>(base),
+    return int(launch(K_OBJ_COUNT, 0, 0.0, 0.0, count_kernel, row_grid(ws.items), dim3(kThreads), stream, rows,
+                      tokens, ignore, mask, seqs, uint32_t(ws.items), reinterpret_cast<int32_t*>(base),
                       by_sequence ? reinterpret_cast<float*>(base + ws.lengths_at) : static_cast<float*>(nullptr)));
 }
 
@@ -382,7 +385,7 @@ extern "C" int mamw_preference_loss(const mamw_rows* logits, const mamw_preferen
     d.smoothing = p->smoothing;
     d.kind = p->kind;
     d.length_average = p->length_average;
-    if ((st = int(launch(K_OBJ_PAIRS, 0, 0.0, 0.0, pairs_kernel, dim3(unsigned(p->sequences / 2)), dim3(kThreads), s,
+    if ((st = int(launch(K_OBJ_PAIRS, 0, 0.0, 0.0, pairs_kernel, row_grid(p->sequences / 2), dim3(kThreads), s,
                          rows, d, static_cast<const float*>(row_logprobs), logprobs, rewards, losses, coef))) != 0)
         return st;
     return int(launch(K_OBJ_RESULT, 1, 0.0, 0.0, mean_kernel, dim3(1), dim3(kThreads), s,

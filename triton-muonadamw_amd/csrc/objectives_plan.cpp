@@ -140,7 +140,8 @@ int check_distill(const mamw_rows* x, const mamw_distill* p, const void* grad, O
     if ((st = check_temperature(p->temperature)) != MAMW_OK) return st;
     if (!isfinite(p->scale)) return MAMW_ERR_HYPER;
     if (p->teacher_lse.data && x->vocab > kMaxTailVocab) return MAMW_ERR_SHAPE;
-    *ws = objective_workspace(count_items(rows), 0, 4 * rows);
+    // Each row's entries (index, probability), its part of the result and what there is to know of its teacher.
+    *ws = objective_workspace((rows + kTeacherRows - 1) / kTeacherRows, 2 * rows * p->k, 8 * rows);
     return MAMW_OK;
 }
 

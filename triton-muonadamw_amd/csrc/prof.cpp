@@ -57,7 +57,7 @@ const char* const kNames[K_COUNT] = {
     "transpose_bf16_kernel", "adamw_bias_kernel", "direct_prep_kernel", "direct_scale_kernel",
     "ns_gemm_direct:gram", "ns_gemm_direct:poly", "ns_gemm_direct:update", "ns_gemm_direct:apply",
     "direct_pack_kernel", "logprobs_kernel", "logits_grad_kernel", "count_kernel", "result_kernel",
-    "policy_kernel", "pairs_kernel", "distill_kernel",
+    "policy_kernel", "pairs_kernel", "distill_kernel", "teacher_kernel",
 };
 
 }  // namespace
