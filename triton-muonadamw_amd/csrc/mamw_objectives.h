@@ -13,7 +13,7 @@ namespace mamw {
 constexpr int kCountRows = 1024;
 // Rows of teacher's entries that one workgroup prepares.
 constexpr int kTeacherRows = 16;
-// Bits of the table of a teacher's indices (128 KiB of LDS at most).
+// Bits of the table of a teacher's indices in rows that are not held whole (128 KiB of LDS at most).
 constexpr int64_t kMaxTailVocab = int64_t(1) << 20;
 
 // A workspace: the rows that count of each sequence (or of each kCountRows or kTeacherRows rows), the length of each

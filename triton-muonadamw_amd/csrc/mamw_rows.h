@@ -445,15 +445,14 @@ struct HeldRow {
             }
     }
 
-    // The wave's statistics.  change(vector, number) is for the vectors that are not held, and with kRest for all: those
-    // held are loaded last then, for the registers.
-    template <typename Change>
-    __device__ __forceinline__ Stats stats(float c, Change change) {
+    // The wave's statistics.  hold(vector, i) is applied to held vector i, change(vector, number) to those that are not
+    // held.  With kRest those held are loaded last, for the registers.
+    template <typename Hold, typename Change>
+    __device__ __forceinline__ Stats stats(float c, Hold hold, Change change) {
         Stats st = no_stats();
         if constexpr (kRest) {
             read_vecs<T, false, false, kThreads_>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
             load_held(row);  // never without a vector
-            each([&](vec_t& x, int n) { change(x, n + int(threadIdx.x)); });
         }
         // In groups, each as its loads arrive: the sum is taken below the thread's largest logit so far and moved when
         // that grows, so that only the reductions are left once the last load is there.
@@ -466,6 +465,7 @@ struct HeldRow {
 #pragma unroll
                 for (int i = q * kGroup; i < (q + 1) * kGroup; ++i) {
                     end_row(i);
+                    hold(v[i], i);
                     float f[kVec<T>];
                     unpack<T>(v[i], f);
 #pragma unroll

@@ -192,12 +192,62 @@ __device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* ld
     return mine;
 }
 
-// kTail: the teacher's entries are taken out of the row (marked in a table of a bit for each entry of the vocabulary)
-// and their sum is added from the gathered logits, so that the sum over all others is not the small difference of two
-// large ones.
+// The teacher's entries of a row that are to be left out of its sum, marked in LDS: a byte for each held vector, all
+// bytes of a thread together, so that it reads them at once (a bit for each element of the vocabulary, looked up for
+// every vector, took 30 us of 178 for 2048 rows of 128256 bf16); a bit for each single element; with kRest a bit for
+// each element of the vocabulary, looked at for the vectors that are not held.
+template <typename T, int kThreads_, int kVecs, bool kRest>
+struct Marks {
+    static constexpr int kWords = (kVecs + 3) / 4;  // of a thread
+    static constexpr int kHeld = kThreads_ * kWords;
+
+    static __host__ __device__ constexpr int words(int vocab) { return kHeld + 1 + (kRest ? (vocab + 31) / 32 : 0); }
+
+    // Marks element j, if `wave` is the wave that holds it, or -1.
+    static __device__ __forceinline__ void set(uint32_t* table, const Span& s, int j, int wave) {
+        const int n = j < s.head ? -1 : (j - s.head) / kVec<T>;
+        const bool is_single = n < 0 || n >= s.vecs;
+        if (wave >= 0 && wave != (is_single ? 0 : n % kThreads_ / 64)) return;
+        if (is_single) {
+            atomicOr(&table[kHeld], 1u << (j < s.head ? j : j - s.vecs * kVec<T>));
+        } else if (n < kVecs * kThreads_) {
+            const int i = n / kThreads_, k = (j - s.head) % kVec<T>;
+            atomicOr(&table[n % kThreads_ * kWords + i / 4], 1u << (i % 4 * 8 + k));
+        } else {
+            atomicOr(&table[kHeld + 1 + (j >> 5)], 1u << (j & 31));
+        }
+    }
+
+    // The elements of v whose bits are set become nothing.
+    static __device__ __forceinline__ void leave_out(vec_t& v, uint32_t bits) {
+        const vec_t none = nothing<T>();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                const uint32_t m = uint32_t(__builtin_amdgcn_sbfe(int32_t(bits), i, 1));
+                v[i] = (v[i] & ~m) | (none[i] & m);
+            } else {
+                const uint32_t lo = uint32_t(__builtin_amdgcn_sbfe(int32_t(bits), 2 * i, 1)) & 0xffffu;
+                const uint32_t hi = uint32_t(__builtin_amdgcn_sbfe(int32_t(bits), 2 * i + 1, 1)) & 0xffff0000u;
+                v[i] = (v[i] & ~(lo | hi)) | (none[i] & (lo | hi));
+            }
+        }
+    }
+
+    // The bits of vector n, not held: elements head + n kVec and on.
+    static __device__ __forceinline__ uint32_t rest(const uint32_t* table, const Span& s, int n, int vocab) {
+        const int j = s.head + n * kVec<T>, w = j >> 5;
+        uint32_t m = table[kHeld + 1 + w] >> (j & 31);
+        if ((j & 31) + kVec<T> > 32 && w + 1 < (vocab + 31) / 32) m |= table[kHeld + 2 + w] << (32 - (j & 31));
+        return m & ((1u << kVec<T>) - 1u);
+    }
+};
+
+// kTail: the teacher's entries are taken out of the row and their sum is added from the gathered logits, so that the
+// sum over all others is not the small difference of two large ones.
 template <typename T, int kThreads_, int kVecs, bool kRest, bool kTail>
 __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
-    Rows x, Distill p, int bits, float4* __restrict__ partials, const float* __restrict__ scale, int unless_one,
+    Rows x, Distill p, float4* __restrict__ partials, const float* __restrict__ scale, int unless_one,
     T* __restrict__ grad) {
     extern __shared__ uint32_t marked[];
     __shared__ Parts lds[kThreads_ / 64];
@@ -229,54 +279,63 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
             probs[e] = p.probs[int64_t(r) * p.k + k];
         }
     }
+    constexpr int kAhead = kTail && !kRest ? 4 : 0;  // of all entries, by each wave
+    int32_t ahead[kAhead + 1];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        ahead[i] = p.index[int64_t(r) * p.k + min(i * 64 + int(threadIdx.x % 64), p.k - 1)];
     const TeacherRow teacher = p.info[r];
     const Counts counted(p.count, p.items, false);
     HeldRow<T, kThreads_, kVecs, kRest> held;
     held.load(row, x.vocab, p.count);
-    if constexpr (kTail) {
-        for (int j = threadIdx.x; j < bits; j += kThreads_) marked[j] = 0;
+    using Mark = Marks<T, kThreads_, kVecs, kRest>;
+    if constexpr (kTail && !kRest) {
+        // Every wave by itself looks through all entries for those in its own vectors: with a barrier here no wave begins
+        // before the last one has started, behind the workgroup before (2048 rows of 128256 bf16: 17 us of 178).
+        const int wave = threadIdx.x / 64;
+#pragma unroll
+        for (int i = 0; i < Mark::kWords; ++i) marked[int(threadIdx.x) * Mark::kWords + i] = 0;
+        if (threadIdx.x == 0) marked[Mark::kHeld] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (ahead[i] >= 0 && i * 64 < p.k) Mark::set(marked, held.span, ahead[i], wave);
+#pragma unroll 1
+        for (int k = kAhead * 64 + int(threadIdx.x % 64); k < p.k; k += 64) {
+            const int j = p.index[int64_t(r) * p.k + k];
+            if (j >= 0) Mark::set(marked, held.span, j, wave);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else if constexpr (kTail) {
+        for (int j = threadIdx.x; j < Mark::words(x.vocab); j += kThreads_) marked[j] = 0;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < kEntries; ++e)
-            if (index[e] >= 0) atomicOr(&marked[index[e] >> 5], 1u << (index[e] & 31));
+            if (index[e] >= 0) Mark::set(marked, held.span, index[e], -1);
+        __syncthreads();
     }
 #pragma unroll
     for (int e = 0; e < kEntries; ++e) xs[e] = raw_at(row + max(index[e], 0));
-    auto take_out = [&](vec_t& v, int n) {
-        if constexpr (kTail) {
-            // the bits of vector n: elements head + n kVec and on
-            const int j = held.span.head + n * kVec<T>;
-            const uint32_t w = j >> 5;
-            if (n >= held.span.vecs) return;  // (the copies of the last vector become nothing later)
-            uint32_t m = marked[w] >> (j & 31);
-            if ((j & 31) + kVec<T> > 32 && int(w) + 1 < bits) m |= marked[w + 1] << (32 - (j & 31));
-            m &= (1u << kVec<T>) - 1u;
-            if (m == 0) return;
-            const vec_t none = nothing<T>();
+    uint32_t mine[Mark::kWords] = {};
+    if constexpr (kTail) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    if (m >> i & 1u) v[i] = none[i];
-                } else {
-                    const uint32_t lo = m >> (2 * i) & 1u ? 0xffffu : 0u, hi = m >> (2 * i + 1) & 1u ? 0xffff0000u : 0u;
-                    v[i] = (v[i] & ~(lo | hi)) | (none[i] & (lo | hi));
-                }
-            }
+        for (int i = 0; i < Mark::kWords; ++i) mine[i] = marked[int(threadIdx.x) * Mark::kWords + i];
+        if (held.has_single() && (marked[Mark::kHeld] >> threadIdx.x & 1u)) held.single_ = raw_nothing<T>();
+    }
+    auto hold = [&](vec_t& v, int i) {
+        if constexpr (kTail) {
+            const uint32_t bits = mine[i / 4] >> (i % 4 * 8) & 0xffu;
+            if (__any(bits != 0)) Mark::leave_out(v, bits);
         }
     };
-    if constexpr (kTail) {
-        __syncthreads();  // all bits are set
-        if constexpr (!kRest)
-            held.each([&](vec_t& v, int n) {
-                take_out(v, n + int(threadIdx.x));
-                // four vectors' bits at a time: all at once would take more registers than there are
-                if (n / kThreads_ % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            });
-        const int j = extra_element<T>(held.span, threadIdx.x);
-        if (int(threadIdx.x) < held.span.extra && (marked[j >> 5] >> (j & 31) & 1u))
-            held.single_ = raw_nothing<T>();
-    }
-    Stats wave = held.stats(x.c, take_out);
+    auto change = [&](vec_t& v, int n) {
+        if constexpr (kTail && kRest)
+            if (n < held.span.vecs) {
+                const uint32_t bits = Mark::rest(marked, held.span, n, x.vocab);
+                if (bits) Mark::leave_out(v, bits);
+            }
+    };
+    Stats wave = held.stats(x.c, hold, change);
     if constexpr (kTail) {
         float x_top = -INFINITY;
 #pragma unroll
@@ -314,7 +373,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
         partials[r] = make_float4((teacher.beyond ? NAN : loss) / count, 0.f, 0.f, 0.f);
     if (g) {
         const float w = teacher.beyond ? NAN : f * p.scale * p.temperature / count;
-        held.write(g, w * share * inv_s, m, x.c, take_out);
+        held.write(g, w * share * inv_s, m, x.c, change);
         __syncthreads();  // then the entries themselves, over what was written there
 #pragma unroll
         for (int e = 0; e < kEntries; ++e)
@@ -375,16 +434,15 @@ int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWor
     d.probs = w.probs;
     d.info = w.info;
     const bool tail = p.teacher_lse.data != nullptr;
-    const int bits = tail ? int((x.vocab + 31) / 32) : 0;
-    const size_t lds = size_t(bits) * 4;
     return with_type(x.type, [&](auto t) {
         using T = decltype(t);
         return with_held_row(x.vocab / kVec<T>, [&](auto n, auto v, auto rest) {
             constexpr int kN = decltype(n)::value, kV = decltype(v)::value;
             constexpr bool kRest = decltype(rest)::value != 0;
+            const size_t lds = tail ? size_t(Marks<T, kN, kV, kRest>::words(int(x.vocab))) * 4 : 0;
             return int(launch_lds(K_OBJ_DISTILL, kN + tail, 0.0, row_bytes(x, grad != nullptr),
                                   tail ? distill_kernel<T, kN, kV, kRest, true> : distill_kernel<T, kN, kV, kRest, false>,
-                                  row_grid(rows.rows), dim3(kN), lds, stream, rows, d, bits, partials, scale,
+                                  row_grid(rows.rows), dim3(kN), lds, stream, rows, d, partials, scale,
                                   unless_one, static_cast<T*>(grad)));
         });
     });
