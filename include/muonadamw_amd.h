@@ -398,7 +398,7 @@ int mamw_policy_grad(const mamw_rows* logits, const mamw_policy* p, const float*
  *     MAMW_SIGMOID: -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h)
  *     MAMW_IPO:     (h / beta - 1 / (2 beta))^2
  *     MAMW_HINGE:   max(0, 1 - h),
- * result[0] = the mean over the pairs.  logprobs = L_s, rewards: one value a sequence.
+ * result[0] = the mean over the pairs (result[1..2] = 0).  logprobs = L_s, rewards: one value a sequence.
  * stats (2 a row) and coef (1 a row) are for mamw_logits_grad.                */
 #define MAMW_SIGMOID 0
 #define MAMW_IPO     1
@@ -425,7 +425,7 @@ int mamw_preference_loss(const mamw_rows* logits, const mamw_preference* p, floa
  *     row = sum_k p_k (log p_k - log q_k)  [+ P log(P / Q)]
  *     P = max(1 - sum_k p_k, 2^-20),  Q = sum of q_j over the other entries
  * (P = 0 where there are no others), result[0] = scale T^2 times the mean over the rows
- * that count.  Entries with a negative index or a logit of -inf are left out.
+ * that count (result[1..2] = 0).  Entries with a negative index or a logit of -inf are left out.
  * k is at most MAMW_MAX_TEACHER; with teacher_lse vocab is at most 2^20.      */
 #define MAMW_MAX_TEACHER 1024
 typedef struct mamw_distill {

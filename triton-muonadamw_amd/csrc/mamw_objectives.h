@@ -20,7 +20,8 @@ constexpr int64_t kMaxTailVocab = int64_t(1) << 20;
 // row's sequence (policy, by sequence) or its teacher's entries, the rows' parts of the result.
 struct ObjectiveWorkspace {
     int64_t items;      // counts
-    size_t lengths_at;  // bytes from the start
+    size_t ticket_at;   // bytes from the start
+    size_t lengths_at;
     size_t partials_at;
     size_t bytes;
 };

@@ -539,13 +539,13 @@ struct Unchanged {
 // of the first 64 counts is apart, to be on its way before a row's.
 struct Counts {
     const int32_t* count;
-    int64_t items;  // at least 1
+    int64_t items;
     bool by_sequence;
     int32_t first;
 
     __device__ __forceinline__ Counts(const int32_t* count_, int64_t items_, bool by_sequence_)
         : count(count_), items(items_), by_sequence(by_sequence_),
-          first(count_[min(int64_t(threadIdx.x % 64), items_ - 1)]) {}
+          first(count_[max(min(int64_t(threadIdx.x % 64), items_ - 1), int64_t(0))]) {}
     __device__ __forceinline__ float one(int32_t n) const { return by_sequence ? float(n > 0) : float(n); }
     __device__ __forceinline__ float all() const {
         const int lane = threadIdx.x % 64;
@@ -554,6 +554,49 @@ struct Counts {
         return fmaxf(wave_sum(n), 1.f);
     }
 };
+
+// ---- the sum over all rows
+
+// Where a launch's workgroups leave their parts of the result.  With a ticket (0 before the launch) the last of them adds
+// up all of them, in the order of their numbers; without one a launch of result_kernel does.
+struct Result {
+    float4* parts;     // NULL: the result is not asked for
+    uint32_t* ticket;
+    uint32_t of;       // workgroups
+    float* result;     // f times the sum of x, the sums of y and z
+    float f;
+};
+
+// By all of a workgroup's threads, at its end.
+__device__ __forceinline__ void put_part(const Result& out, uint32_t i, float x, float y, float z) {
+    if (!out.parts || threadIdx.x >= 64) return;
+    if (!out.ticket) {
+        if (threadIdx.x == 0) out.parts[i] = make_float4(x, y, z, 0.f);
+        return;
+    }
+    uint32_t before = 0;
+    if (threadIdx.x == 0) {
+        float* part = reinterpret_cast<float*>(out.parts + i);
+        __hip_atomic_store(part, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(part + 1, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(part + 2, z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        before = __hip_atomic_fetch_add(out.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (uint32_t(__builtin_amdgcn_readfirstlane(int(before))) != out.of - 1) return;
+    float sum[3] = {0.f, 0.f, 0.f};
+    for (uint32_t k = threadIdx.x; k < out.of; k += 64) {
+        const float* part = reinterpret_cast<const float*>(out.parts + k);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) sum[j] += __hip_atomic_load(part + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) sum[j] = wave_sum(sum[j]);
+    if (threadIdx.x == 0) {
+        out.result[0] = sum[0] * out.f;
+        out.result[1] = sum[1];
+        out.result[2] = sum[2];
+    }
+}
 
 // ---- launches
 
@@ -621,9 +664,25 @@ inline dim3 row_grid(int64_t rows) {
     return rows <= int64_t(most) ? dim3(unsigned(rows)) : dim3(most, unsigned((rows + most - 1) / most));
 }
 
+// Up to this many rows the last workgroup adds up the result; above, where the launch is long against another, a kernel
+// of its own does, and the workgroups need not wait for each other's memory.
+constexpr int64_t kTicketRows = 1024;
+
+// Where the rows' parts of `result` go; `launched`: the ticket is cleared by a launch before.
+inline Result make_result(const ObjectiveWorkspace& ws, char* base, int64_t rows, bool launched, float f, float* result) {
+    Result out;
+    out.parts = reinterpret_cast<float4*>(base + ws.partials_at);
+    out.ticket = launched && rows <= kTicketRows ? reinterpret_cast<uint32_t*>(base + ws.ticket_at) : nullptr;
+    out.of = uint32_t(rows);
+    out.result = result;
+    out.f = f;
+    return out;
+}
+
 // Defined in objectives.hip.
 int launch_count(const Rows& rows, const PerRow& tokens, int64_t ignore, const PerRow& mask, const Sequences& seqs,
                  const ObjectiveWorkspace& ws, bool by_sequence, char* base, hipStream_t stream);
-int launch_result(const ObjectiveWorkspace& ws, char* base, int64_t rows, float f, float* result, hipStream_t stream);
+// result_kernel, where the workgroups had no ticket.
+int launch_result(const Result& out, hipStream_t stream);
 
 }  // namespace mamw

@@ -41,7 +41,8 @@ template <int kPerLane, bool kTail>
 __global__ __launch_bounds__(64 * kTeacherRows) void teacher_kernel(Rows x, TeacherArgs a, int32_t* __restrict__ index,
                                                                     float* __restrict__ probs,
                                                                     TeacherRow* __restrict__ info, uint32_t items,
-                                                                    int32_t* __restrict__ count) {
+                                                                    int32_t* __restrict__ count,
+                                                                    uint32_t* __restrict__ ticket) {
     __shared__ uint32_t seen_bits[kTeacherRows][kSeenBits / 32];
     __shared__ int active[kTeacherRows];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
@@ -146,6 +147,7 @@ __global__ __launch_bounds__(64 * kTeacherRows) void teacher_kernel(Rows x, Teac
         int n = 0;
         for (int w = 0; w < kTeacherRows; ++w) n += active[w];
         count[item] = n;
+        if (item == 0) *ticket = 0;
     }
 }
 
@@ -247,7 +249,7 @@ struct Marks {
 // sum over all others is not the small difference of two large ones.
 template <typename T, int kThreads_, int kVecs, bool kRest, bool kTail>
 __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
-    Rows x, Distill p, float4* __restrict__ partials, const float* __restrict__ scale, int unless_one,
+    Rows x, Distill p, Result out, const float* __restrict__ scale, int unless_one,
     T* __restrict__ grad) {
     extern __shared__ uint32_t marked[];
     __shared__ Parts lds[kThreads_ / 64];
@@ -259,8 +261,8 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
     const Place at = place(x, r);
     T* g = grad ? grad + int64_t(r) * x.vocab : nullptr;
     if (!load_mask(p.mask, at)) {
-        if (partials && threadIdx.x == 0) partials[r] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (g) zero_row(g, x.vocab, kThreads_);
+        put_part(out, r, 0.f, 0.f, 0.f);
         return;
     }
     const T* row = row_of<T>(x, at);
@@ -369,8 +371,6 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
             share = 1.f - rest_p / rest_q;
         }
     }
-    if (partials && threadIdx.x == 0)
-        partials[r] = make_float4((teacher.beyond ? NAN : loss) / count, 0.f, 0.f, 0.f);
     if (g) {
         const float w = teacher.beyond ? NAN : f * p.scale * p.temperature / count;
         held.write(g, w * share * inv_s, m, x.c, change);
@@ -380,25 +380,26 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
             if (index[e] >= 0)
                 g[index[e]] = narrow<T>(w * (in * inv_s * __builtin_amdgcn_exp2f(below(xs[e].value(), m, x.c)) - probs[e]));
     }
+    put_part(out, r, (teacher.beyond ? NAN : loss) / count, 0.f, 0.f);
 }
 
 // ---- launches
 
 struct DistillWorkspace {
     int32_t* count;
+    uint32_t* ticket;
     int32_t* index;
     float* probs;
-    float4* partials;
     TeacherRow* info;
 };
 
 DistillWorkspace parts_of(const ObjectiveWorkspace& ws, char* base, int64_t rows, int64_t k) {
     DistillWorkspace w;
     w.count = reinterpret_cast<int32_t*>(base);
+    w.ticket = reinterpret_cast<uint32_t*>(base + ws.ticket_at);
     w.index = reinterpret_cast<int32_t*>(base + ws.lengths_at);
     w.probs = reinterpret_cast<float*>(w.index + rows * k);
-    w.partials = reinterpret_cast<float4*>(base + ws.partials_at);
-    w.info = reinterpret_cast<TeacherRow*>(w.partials + rows);
+    w.info = reinterpret_cast<TeacherRow*>(reinterpret_cast<float4*>(base + ws.partials_at) + rows);
     return w;
 }
 
@@ -413,14 +414,14 @@ int launch_teacher(const mamw_rows& x, const mamw_distill& p, const ObjectiveWor
         return int(launch(K_OBJ_TEACHER, kPerLane, 0.0, 0.0,
                           p.teacher_lse.data ? teacher_kernel<kPerLane, true> : teacher_kernel<kPerLane, false>,
                           row_grid(ws.items), dim3(64 * kTeacherRows), stream, rows, a, w.index, w.probs, w.info,
-                          uint32_t(ws.items), w.count));
+                          uint32_t(ws.items), w.count, w.ticket));
     };
     return p.k <= 64 ? go(Int<1>()) : p.k <= 128 ? go(Int<2>()) : p.k <= 256 ? go(Int<4>())
          : p.k <= 512 ? go(Int<8>()) : go(Int<16>());
 }
 
 int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWorkspace& ws, const DistillWorkspace& w,
-                   float4* partials, const float* scale, int unless_one, void* grad, hipStream_t stream) {
+                   const Result& out, const float* scale, int unless_one, void* grad, hipStream_t stream) {
     const Rows rows = make_rows(x, p.temperature);
     if (rows.rows == 0) return MAMW_OK;
     Distill d;
@@ -442,7 +443,7 @@ int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWor
             const size_t lds = tail ? size_t(Marks<T, kN, kV, kRest>::words(int(x.vocab))) * 4 : 0;
             return int(launch_lds(K_OBJ_DISTILL, kN + tail, 0.0, row_bytes(x, grad != nullptr),
                                   tail ? distill_kernel<T, kN, kV, kRest, true> : distill_kernel<T, kN, kV, kRest, false>,
-                                  row_grid(rows.rows), dim3(kN), lds, stream, rows, d, partials, scale,
+                                  row_grid(rows.rows), dim3(kN), lds, stream, rows, d, out, scale,
                                   unless_one, static_cast<T*>(grad)));
         });
     });
@@ -473,8 +474,9 @@ extern "C" int mamw_distill_loss(const mamw_rows* logits, const mamw_distill* p,
     const DistillWorkspace w = parts_of(ws, base, rows, p->k);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if ((st = launch_teacher(*logits, *p, ws, w, s)) != MAMW_OK) return st;
-    if ((st = launch_distill(*logits, *p, ws, w, w.partials, nullptr, 0, grad, s)) != MAMW_OK) return st;
-    return launch_result(ws, base, rows, p->scale * p->temperature * p->temperature, result, s);
+    const Result out = make_result(ws, base, rows, rows > 0, p->scale * p->temperature * p->temperature, result);
+    if ((st = launch_distill(*logits, *p, ws, w, out, nullptr, 0, grad, s)) != MAMW_OK) return st;
+    return launch_result(out, s);
 }
 
 extern "C" int mamw_distill_grad(const mamw_rows* logits, const mamw_distill* p, const float* scale, int unless_one,
@@ -486,5 +488,5 @@ extern "C" int mamw_distill_grad(const mamw_rows* logits, const mamw_distill* p,
     const int64_t rows = logits->outer * logits->inner;
     if (!scale || (!grad && rows > 0)) return MAMW_ERR_NULL;
     const DistillWorkspace w = parts_of(ws, static_cast<char*>(workspace), rows, p->k);
-    return launch_distill(*logits, *p, ws, w, nullptr, scale, unless_one, grad, static_cast<hipStream_t>(stream));
+    return launch_distill(*logits, *p, ws, w, Result(), scale, unless_one, grad, static_cast<hipStream_t>(stream));
 }

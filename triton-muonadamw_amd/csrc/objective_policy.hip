@@ -17,7 +17,7 @@ struct Policy {
 
 template <typename T, int kThreads_, int kVecs, bool kRest>
 __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
-    Rows x, Policy p, float* __restrict__ logprobs, float4* __restrict__ partials, const float* __restrict__ scale,
+    Rows x, Policy p, float* __restrict__ logprobs, Result out, const float* __restrict__ scale,
     int unless_one, T* __restrict__ grad) {
     __shared__ Stats lds[kThreads_ / 64];
     const float f = scale ? *scale : 1.f;
@@ -30,8 +30,8 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
     const float length = p.by_sequence ? p.lengths[r] : 1.f;  // 0: in no sequence
     if (token == p.ignore || length == 0.f) {
         if (logprobs && threadIdx.x == 0) logprobs[r] = 0.f;
-        if (partials && threadIdx.x == 0) partials[r] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (g) zero_row(g, x.vocab, kThreads_);
+        put_part(out, r, 0.f, 0.f, 0.f);
         return;
     }
     const T* row = row_of<T>(x, at);
@@ -58,10 +58,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
         loss += p.kl_coef * kl;
         slope -= p.kl_coef * e;
     }
-    if (threadIdx.x == 0) {
-        if (logprobs) logprobs[r] = lp;
-        if (partials) partials[r] = make_float4(w * p.scale * loss, w * kl, clipped ? w : 0.f, 0.f);
-    }
+    if (logprobs && threadIdx.x == 0) logprobs[r] = lp;
     if (g) {
         const float a = beyond ? NAN : f * p.scale * w * slope * x.inv_t, b = -a / st.s;
         held.write(g, b, st.m, x.c, Unchanged());
@@ -69,10 +66,11 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
         if (!beyond && int(threadIdx.x) == owner_of<T>(held.span, int(token), kThreads_))
             g[token] = narrow<T>(a + b * __builtin_amdgcn_exp2f(below(xt, st.m, x.c)));
     }
+    put_part(out, r, w * p.scale * loss, w * kl, clipped ? w : 0.f);
 }
 
 int launch_policy(const mamw_rows& x, const mamw_policy& p, const ObjectiveWorkspace& ws, float* logprobs,
-                  float4* partials, const float* scale, int unless_one, void* grad, char* base, hipStream_t stream) {
+                  const Result& out, const float* scale, int unless_one, void* grad, char* base, hipStream_t stream) {
     const Rows rows = make_rows(x, p.temperature);
     if (rows.rows == 0) return MAMW_OK;
     Policy d;
@@ -95,7 +93,7 @@ int launch_policy(const mamw_rows& x, const mamw_policy& p, const ObjectiveWorks
             constexpr int kN = decltype(n)::value;
             return int(launch(K_OBJ_POLICY, kN, 0.0, row_bytes(x, grad != nullptr),
                               policy_kernel<T, kN, decltype(v)::value, decltype(rest)::value != 0>,
-                              row_grid(rows.rows), dim3(kN), stream, rows, d, logprobs, partials,
+                              row_grid(rows.rows), dim3(kN), stream, rows, d, logprobs, out,
                               scale, unless_one, static_cast<T*>(grad)));
         });
     });
@@ -123,14 +121,14 @@ extern "C" int mamw_policy_loss(const mamw_rows* logits, const mamw_policy* p, f
     const Rows rows = make_rows(*logits, p->temperature);
     if (!result || (rows.rows > 0 && !logprobs)) return MAMW_ERR_NULL;
     char* base = static_cast<char*>(workspace);
-    float4* partials = reinterpret_cast<float4*>(base + ws.partials_at);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const PerRow none = {};
     if ((st = launch_count(rows, make_per_row(p->tokens), p->ignore_index, none, {p->offsets, p->sequences}, ws,
                            p->by_sequence, base, s)) != MAMW_OK)
         return st;
-    if ((st = launch_policy(*logits, *p, ws, logprobs, partials, nullptr, 0, grad, base, s)) != MAMW_OK) return st;
-    return launch_result(ws, base, rows.rows, 1.f, result, s);
+    const Result out = make_result(ws, base, rows.rows, ws.items > 0 && rows.rows > 0, 1.f, result);
+    if ((st = launch_policy(*logits, *p, ws, logprobs, out, nullptr, 0, grad, base, s)) != MAMW_OK) return st;
+    return launch_result(out, s);
 }
 
 extern "C" int mamw_policy_grad(const mamw_rows* logits, const mamw_policy* p, const float* scale, int unless_one,
@@ -140,6 +138,6 @@ extern "C" int mamw_policy_grad(const mamw_rows* logits, const mamw_policy* p, c
     if (st != MAMW_OK) return st;
     if ((st = check_workspace(ws, workspace, workspace_bytes)) != MAMW_OK) return st;
     if (!scale || (!grad && logits->outer * logits->inner > 0)) return MAMW_ERR_NULL;
-    return launch_policy(*logits, *p, ws, nullptr, nullptr, scale, unless_one, grad, static_cast<char*>(workspace),
+    return launch_policy(*logits, *p, ws, nullptr, Result(), scale, unless_one, grad, static_cast<char*>(workspace),
                          static_cast<hipStream_t>(stream));
 }

@@ -17,7 +17,8 @@ template <typename T, int kThreads_, bool kEntropy>
 __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow tokens, int64_t ignore,
                                                              float* __restrict__ logprobs,
                                                              float* __restrict__ entropy, float* __restrict__ stats,
-                                                             float* __restrict__ coef) {
+                                                             float* __restrict__ coef,
+                                                             uint32_t* __restrict__ ticket) {
     __shared__ Stats lds[2][kThreads_ / 64];
     const uint32_t r = row_of_block();
     if (r >= uint32_t(x.rows)) return;
@@ -25,6 +26,7 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
     const int64_t token = load_int(tokens, offset(tokens, at));
     float lp = 0.f, h = 0.f;
     if (coef && threadIdx.x == 0) coef[r] = 0.f;  // of rows outside all sequences
+    if (ticket && r == 0 && threadIdx.x == 0) *ticket = 0;
     if (token != ignore) {
         const T* row = row_of<T>(x, at);
         const float xt = chosen(row, token, x.vocab);
@@ -147,7 +149,8 @@ __device__ __forceinline__ bool counts(const Rows& x, const PerRow& tokens, int6
 // (lengths NULL), of the kCountRows rows from i kCountRows on.
 __global__ __launch_bounds__(kThreads) void count_kernel(Rows x, PerRow tokens, int64_t ignore, PerRow mask,
                                                          Sequences seqs, uint32_t items, int32_t* __restrict__ count,
-                                                         float* __restrict__ lengths) {
+                                                         float* __restrict__ lengths,
+                                                         uint32_t* __restrict__ ticket) {
     __shared__ float lds[kWaves];
     const uint32_t item = row_of_block();
     if (item >= items) return;
@@ -158,6 +161,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(Rows x, PerRow tokens, 
     // below 2^24 a thread; exact as floats where the sum is, too, else the weight's last bit
     const float all = block_sum(Floats<1>{{float(n)}}, lds).v[0];
     if (threadIdx.x == 0) count[item] = int32_t(all);
+    if (item == 0 && threadIdx.x == 0) *ticket = 0;
     if (lengths)
         for (int64_t r = from + threadIdx.x; r < to; r += kThreads) lengths[r] = all;
 }
@@ -167,23 +171,22 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(float* __restrict__ x, i
     if (i < n) x[i] = 0.f;
 }
 
-// result[0..2]: the sums of the rows' parts, always in the same order.
+// The sums of the rows' parts, always in the same order.
 constexpr int kResultThreads = 1024;
-__global__ __launch_bounds__(kResultThreads) void result_kernel(const float4* __restrict__ parts, int rows, float f,
-                                                                float* __restrict__ result) {
+__global__ __launch_bounds__(kResultThreads) void result_kernel(Result out) {
     __shared__ float lds[kResultThreads / 64 * 3];
     Floats<3> sum = {{0.f, 0.f, 0.f}};
-    for (int i = threadIdx.x; i < rows; i += kResultThreads) {
-        const float4 x = parts[i];
+    for (uint32_t i = threadIdx.x; i < out.of; i += kResultThreads) {
+        const float4 x = out.parts[i];
         sum.v[0] += x.x;
         sum.v[1] += x.y;
         sum.v[2] += x.z;
     }
     sum = block_sum<3, kResultThreads>(sum, lds);
     if (threadIdx.x == 0) {
-        result[0] = sum.v[0] * f;
-        result[1] = sum.v[1];
-        result[2] = sum.v[2];
+        out.result[0] = sum.v[0] * out.f;
+        out.result[1] = sum.v[1];
+        out.result[2] = sum.v[2];
     }
 }
 
@@ -198,33 +201,43 @@ struct Preference {
     int kind, length_average;
 };
 
-// One workgroup a pair: the sums over both sequences, the pair's loss and the rows' coefficients.
+// The sum over the workgroup in 64 bits.
+__device__ __forceinline__ double block_sum64(double x, double* lds) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
+    __syncthreads();
+    x = lds[0];
+    for (int w = 1; w < kWaves; ++w) x += lds[w];
+    return x;
+}
+
+// One workgroup a pair: the sums over both sequences, the pair's loss and the rows' coefficients.  The sums are of a
+// thousand log-probabilities, and what counts is how little they differ from a reference's: in 64 bits, as is the
+// margin.
 __global__ __launch_bounds__(kThreads) void pairs_kernel(Rows x, Preference p, const float* __restrict__ row_logprobs,
                                                          float* __restrict__ logprobs, float* __restrict__ rewards,
-                                                         float* __restrict__ losses, float* __restrict__ coef) {
-    __shared__ float lds[kWaves * 2];
+                                                         Result out, float* __restrict__ coef) {
+    __shared__ double lds[kWaves];
     const int64_t pairs = p.seqs.count / 2, i = row_of_block();
     if (i >= pairs) return;
     const PerRow none = {};
     int64_t from[2], to[2];
-    // Sums of a thousand log-probabilities, whose differences to a reference's are what counts: in 64 bits, as is a
-    // reward until it is written.
-    double total[2];
-    float n[2];
+    double total[2], n[2], reward[2];
     for (int k = 0; k < 2; ++k) {
         sequence_rows(p.seqs, x, i + k * pairs, &from[k], &to[k]);
-        Floats<2> sum = {{0.f, 0.f}};
+        double sum = 0.0;
+        int count = 0;
         for (int64_t r = from[k] + threadIdx.x; r < to[k]; r += kThreads) {
-            sum.v[0] += row_logprobs[r];
-            sum.v[1] += counts(x, p.tokens, p.ignore, none, uint32_t(r));
+            sum += row_logprobs[r];
+            count += counts(x, p.tokens, p.ignore, none, uint32_t(r));
         }
-        sum = block_sum(sum, lds);
-        n[k] = p.length_average ? fmaxf(sum.v[1], 1.f) : 1.f;
-        total[k] = sum.v[0] / n[k];
+        n[k] = p.length_average ? fmax(block_sum64(count, lds), 1.0) : 1.0;
+        total[k] = block_sum64(sum, lds) / n[k];
+        reward[k] = double(p.beta) * (total[k] - (p.ref ? p.ref[i + k * pairs] : 0.f));
     }
-    const float reward0 = p.beta * (total[0] - (p.ref ? p.ref[i] : 0.f));
-    const float reward1 = p.beta * (total[1] - (p.ref ? p.ref[i + pairs] : 0.f));
-    const float h = reward0 - reward1;
+    const float h = float(reward[0] - reward[1]);
     float loss, slope;  // d loss / d h
     if (p.kind == MAMW_SIGMOID) {
         const float soft = log1pf(expf(-fabsf(h)));  // -log sigmoid(|h|)
@@ -238,33 +251,23 @@ __global__ __launch_bounds__(kThreads) void pairs_kernel(Rows x, Preference p, c
         loss = h < 1.f ? 1.f - h : h >= 1.f ? 0.f : h;  // NaN stays
         slope = h < 1.f ? -1.f : h >= 1.f ? 0.f : h;
     }
-    if (threadIdx.x == 0) {
-        logprobs[i] = total[0];
-        logprobs[i + pairs] = total[1];
-        rewards[i] = reward0;
-        rewards[i + pairs] = reward1;
-        losses[i] = loss;
+    if (threadIdx.x < 2) {
+        const int k = threadIdx.x;
+        logprobs[i + k * pairs] = float(k ? total[1] : total[0]);
+        rewards[i + k * pairs] = float(k ? reward[1] : reward[0]);
     }
     if (coef)
         for (int k = 0; k < 2; ++k) {
-            const float c = (k ? -slope : slope) * p.beta / (float(pairs) * n[k]);
+            const float c = (k ? -slope : slope) * p.beta / (float(pairs) * float(n[k]));
             for (int64_t r = from[k] + threadIdx.x; r < to[k]; r += kThreads) coef[r] = c;
         }
-}
-
-__global__ __launch_bounds__(kThreads) void mean_kernel(const float* __restrict__ x, int64_t n,
-                                                        float* __restrict__ result) {
-    __shared__ float lds[kWaves];
-    float sum = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) sum += x[i];
-    sum = block_sum(Floats<1>{{sum}}, lds).v[0];
-    if (threadIdx.x == 0) result[0] = sum / float(n);
+    put_part(out, uint32_t(i), loss, 0.f, 0.f);
 }
 
 // ---- launches
 
 int launch_logprobs(const mamw_rows& x, const mamw_per_row& tokens, int64_t ignore, float temperature,
-                    float* logprobs, float* entropy, float* stats, float* coef, hipStream_t stream) {
+                    float* logprobs, float* entropy, float* stats, float* coef, uint32_t* ticket, hipStream_t stream) {
     const Rows rows = make_rows(x, temperature);
     return with_type(x.type, [&](auto t) {
         using T = decltype(t);
@@ -273,7 +276,7 @@ int launch_logprobs(const mamw_rows& x, const mamw_per_row& tokens, int64_t igno
             return int(launch(K_OBJ_LOGPROBS, entropy ? 1 : 0, 0.0, row_bytes(x, false),
                               entropy ? logprobs_kernel<T, kN, true> : logprobs_kernel<T, kN, false>,
                               row_grid(rows.rows), dim3(kN), stream, rows, make_per_row(tokens), ignore,
-                              logprobs, entropy, stats, coef));
+                              logprobs, entropy, stats, coef, ticket));
         };
         // By the vocabulary alone, so that a row's result does not depend on how many there are.
         const int64_t vecs = x.vocab / kVec<T>;
@@ -297,12 +300,13 @@ int launch_count(const Rows& rows, const PerRow& tokens, int64_t ignore, const P
     if (ws.items == 0) return MAMW_OK;
     return int(launch(K_OBJ_COUNT, 0, 0.0, 0.0, count_kernel, row_grid(ws.items), dim3(kThreads), stream, rows,
                       tokens, ignore, mask, seqs, uint32_t(ws.items), reinterpret_cast<int32_t*>(base),
-                      by_sequence ? reinterpret_cast<float*>(base + ws.lengths_at) : static_cast<float*>(nullptr)));
+                      by_sequence ? reinterpret_cast<float*>(base + ws.lengths_at) : static_cast<float*>(nullptr),
+                      reinterpret_cast<uint32_t*>(base + ws.ticket_at)));
 }
 
-int launch_result(const ObjectiveWorkspace& ws, char* base, int64_t rows, float f, float* result, hipStream_t stream) {
-    return int(launch(K_OBJ_RESULT, 0, 0.0, 0.0, result_kernel, dim3(1), dim3(kResultThreads), stream,
-                      reinterpret_cast<const float4*>(base + ws.partials_at), int(rows), f, result));
+int launch_result(const Result& out, hipStream_t stream) {
+    if (out.ticket) return MAMW_OK;
+    return int(launch(K_OBJ_RESULT, 0, 0.0, 0.0, result_kernel, dim3(1), dim3(kResultThreads), stream, out));
 }
 
 }  // namespace mamw
@@ -321,7 +325,7 @@ extern "C" int mamw_token_logprobs(const mamw_rows* logits, const mamw_per_row* 
     if (!some) return MAMW_OK;
     if (!logprobs) return MAMW_ERR_NULL;
     return launch_logprobs(*logits, *tokens, ignore_index, temperature, logprobs, entropy, stats,
-                           nullptr, static_cast<hipStream_t>(stream));
+                           nullptr, nullptr, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int mamw_logits_grad(const mamw_rows* logits, const mamw_per_row* tokens, int64_t ignore_index,
@@ -371,11 +375,20 @@ extern "C" int mamw_preference_loss(const mamw_rows* logits, const mamw_preferen
     const Rows rows = make_rows(*logits, p->temperature);
     char* base = static_cast<char*>(workspace);
     float* row_logprobs = reinterpret_cast<float*>(base + ws.lengths_at);
-    float* losses = reinterpret_cast<float*>(base + ws.partials_at);
+    uint32_t* ticket = reinterpret_cast<uint32_t*>(base + ws.ticket_at);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (rows.rows > 0 && (st = launch_logprobs(*logits, p->tokens, p->ignore_index, p->temperature, row_logprobs,
-                                               nullptr, stats, coef, s)) != MAMW_OK)
-        return st;
+    st = rows.rows > 0 ? launch_logprobs(*logits, p->tokens, p->ignore_index, p->temperature, row_logprobs, nullptr, stats,
+                                         coef, ticket, s)
+                       : int(launch(K_OBJ_COUNT, 1, 0.0, 0.0, zero_kernel, dim3(1), dim3(kThreads), s,
+                                    reinterpret_cast<float*>(ticket), int64_t(1)));
+    if (st != MAMW_OK) return st;
+    const int64_t pairs = p->sequences / 2;
+    Result out;
+    out.parts = reinterpret_cast<float4*>(base + ws.partials_at);
+    out.ticket = ticket;
+    out.of = uint32_t(pairs);
+    out.result = result;
+    out.f = 1.f / float(pairs);
     Preference d;
     d.tokens = make_per_row(p->tokens);
     d.ignore = p->ignore_index;
@@ -385,9 +398,6 @@ extern "C" int mamw_preference_loss(const mamw_rows* logits, const mamw_preferen
     d.smoothing = p->smoothing;
     d.kind = p->kind;
     d.length_average = p->length_average;
-    if ((st = int(launch(K_OBJ_PAIRS, 0, 0.0, 0.0, pairs_kernel, row_grid(p->sequences / 2), dim3(kThreads), s,
-                         rows, d, static_cast<const float*>(row_logprobs), logprobs, rewards, losses, coef))) != 0)
-        return st;
-    return int(launch(K_OBJ_RESULT, 1, 0.0, 0.0, mean_kernel, dim3(1), dim3(kThreads), s,
-                      static_cast<const float*>(losses), p->sequences / 2, result));
+    return int(launch(K_OBJ_PAIRS, 0, 0.0, 0.0, pairs_kernel, row_grid(pairs), dim3(kThreads), s, rows, d,
+                      static_cast<const float*>(row_logprobs), logprobs, rewards, out, coef));
 }

@@ -464,14 +464,15 @@ PyObject* preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard device(logits.device());
         const Tensor workspace = bytes(need, logits);
-        loss = floats({}, logits);
+        const Tensor result = floats({3}, logits);
+        loss = result.select(0, 0);
         logprobs = floats({count}, logits);
         rewards = floats({count}, logits);
         if (grad) {
             stats = floats({rows.outer, rows.inner, 2}, logits);
             coef = floats(logits.sizes().slice(0, logits.dim() - 1), logits);
         }
-        check(mamw_preference_loss(&rows, &p, ptr<float>(loss), ptr<float>(logprobs), ptr<float>(rewards),
+        check(mamw_preference_loss(&rows, &p, ptr<float>(result), ptr<float>(logprobs), ptr<float>(rewards),
                                    ptr<float>(stats), ptr<float>(coef), ptr(workspace), workspace.numel(),
                                    stream_of(logits)),
               "preference_loss");

@@ -28,7 +28,8 @@ size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 ObjectiveWorkspace objective_workspace(int64_t items, int64_t lengths, int64_t partials) {
     ObjectiveWorkspace w;
     w.items = items;
-    w.lengths_at = round_up(size_t(items) * 4);
+    w.ticket_at = round_up(size_t(items) * 4);
+    w.lengths_at = w.ticket_at + 256;
     w.partials_at = w.lengths_at + round_up(size_t(lengths) * 4);
     w.bytes = w.partials_at + round_up(size_t(partials) * 4);
     return w;
@@ -120,7 +121,7 @@ int check_preference(const mamw_rows* x, const mamw_preference* p, ObjectiveWork
     if (p->kind < MAMW_SIGMOID || p->kind > MAMW_HINGE || p->reserved) return MAMW_ERR_HYPER;
     if (p->kind != MAMW_SIGMOID && p->smoothing != 0.f) return MAMW_ERR_HYPER;
     // The rows' log-probabilities, and one loss a pair.
-    *ws = objective_workspace(0, rows, p->sequences / 2);
+    *ws = objective_workspace(0, rows, 2 * p->sequences);
     return MAMW_OK;
 }
 
