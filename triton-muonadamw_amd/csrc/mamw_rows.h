@@ -232,9 +232,15 @@ __device__ __forceinline__ int owner_of(const Span& s, int j, int threads) {
 //
 // Vector `thread` of those from `first` on, with `first` the same for the whole workgroup: scalar address and 32-bit
 // offset, no registers for sixteen 64-bit addresses.
+// kKeep: through the caches all the same, for who reads the row next.
+template <bool kKeep = false>
 __device__ __forceinline__ vec_t load_vec(const void* vecs, int first, int thread) {
     const char* at = static_cast<const char*>(vecs) + int64_t(first) * 16;
-    return __builtin_nontemporal_load(reinterpret_cast<const vec_t*>(at + uint32_t(thread) * 16u));
+    const vec_t* from = reinterpret_cast<const vec_t*>(at + uint32_t(thread) * 16u);
+    if constexpr (kKeep)
+        return *from;
+    else
+        return __builtin_nontemporal_load(from);
 }
 __device__ __forceinline__ void store_vec(void* vecs, int first, int thread, vec_t v) {
     // at any element: the gradient's rows may lie otherwise than the logits'
@@ -328,7 +334,7 @@ __device__ __forceinline__ bool quick_holds(const Stats& st) {
 }
 
 // The statistics of vectors from + threadIdx.x, + kThreads_, ... below `to`; change(v, n) is applied to vector n.
-template <typename T, bool kEntropy, bool kQuick, int kThreads_, typename Change>
+template <typename T, bool kEntropy, bool kQuick, int kThreads_, bool kKeep = false, typename Change>
 __device__ __forceinline__ void read_vecs(Stats& st, const void* vecs, int from, int to, float c, Change change) {
     constexpr int kUnroll = 4;
     const int t = threadIdx.x;
@@ -336,7 +342,7 @@ __device__ __forceinline__ void read_vecs(Stats& st, const void* vecs, int from,
     int n = from;
     for (; n + kUnroll * kThreads_ <= to; n += kUnroll * kThreads_) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) v[u] = load_vec(vecs, n + u * kThreads_, t);
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_vec<kKeep>(vecs, n + u * kThreads_, t);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) change(v[u], n + u * kThreads_ + t);
         add_vecs<T, kEntropy, kQuick, kUnroll>(st, v, c);
@@ -345,7 +351,7 @@ __device__ __forceinline__ void read_vecs(Stats& st, const void* vecs, int from,
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         const int first = n + u * kThreads_;
-        v[u] = first + t < to ? load_vec(vecs, first, t) : nothing<T>();
+        v[u] = first + t < to ? load_vec<kKeep>(vecs, first, t) : nothing<T>();
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)

@@ -18,7 +18,7 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
                                                              float* __restrict__ logprobs,
                                                              float* __restrict__ entropy, float* __restrict__ stats,
                                                              float* __restrict__ coef,
-                                                             uint32_t* __restrict__ ticket) {
+                                                             uint32_t* __restrict__ ticket, uint32_t keep_from) {
     __shared__ Stats lds[2][kThreads_ / 64];
     const uint32_t r = row_of_block();
     if (r >= uint32_t(x.rows)) return;
@@ -38,7 +38,10 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
                 st.m = widen(row[extra_element<T>(span, threadIdx.x)]);
                 add<kEntropy>(st, st.m, reference(st.m), x.c);
             }
-            read_vecs<T, kEntropy, kQuick, kThreads_>(st, row + span.head, 0, span.vecs, x.c, Unchanged());
+            if (kQuick && r >= keep_from)
+                read_vecs<T, kEntropy, kQuick, kThreads_, true>(st, row + span.head, 0, span.vecs, x.c, Unchanged());
+            else
+                read_vecs<T, kEntropy, kQuick, kThreads_>(st, row + span.head, 0, span.vecs, x.c, Unchanged());
             return over_block<kEntropy, kThreads_>(over_wave<kEntropy>(st, x.c), x.c, lds[!kQuick]);
         };
         Stats st = stats_of_row(Int<1>());
@@ -60,9 +63,14 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
 // ---- the gradient from statistics at hand
 
 // A workgroup takes kGradVecs vectors of one row: it waits for nothing, so short-lived ones in great number come
-// nearest to a copy.
-constexpr int kGradUnroll = 4;
+// nearest to a copy (6000 x 50257 bf16: 224 us with eight vectors a thread, 209 with four, 198 with two, 204 with
+// one).  Rows are taken from the last: those the statistics were taken of last are still in the memory-side cache of 256
+// MB (198 -> 183 us).
+constexpr int kGradUnroll = 2;
 constexpr int kGradVecs = kThreads * kGradUnroll;
+// Logits that the statistics leave there.  More than it holds, since of rows that do not count nothing is read; all of
+// them cost 10 us of 78 there and gain nothing here.
+constexpr double kKeptBytes = 400e6;
 
 template <typename T, bool kEntropy>
 __global__ __launch_bounds__(kThreads) void logits_grad_kernel(Rows x, PerRow tokens, int64_t ignore,
@@ -73,7 +81,8 @@ __global__ __launch_bounds__(kThreads) void logits_grad_kernel(Rows x, PerRow to
                                                                T* __restrict__ grad) {
     const float f = (scale ? *scale : 1.f) * x.inv_t;
     const uint32_t part = blockIdx.x;
-    for (uint32_t r = blockIdx.y; r < uint32_t(x.rows); r += gridDim.y) {
+    for (uint32_t back = blockIdx.y; back < uint32_t(x.rows); back += gridDim.y) {
+        const uint32_t r = uint32_t(x.rows) - 1 - back;
         const Place at = place(x, r);
         const int64_t token = load_int(tokens, offset(tokens, at));
         T* g = grad + int64_t(r) * x.vocab;
@@ -269,6 +278,10 @@ __global__ __launch_bounds__(kThreads) void pairs_kernel(Rows x, Preference p, c
 int launch_logprobs(const mamw_rows& x, const mamw_per_row& tokens, int64_t ignore, float temperature,
                     float* logprobs, float* entropy, float* stats, float* coef, uint32_t* ticket, hipStream_t stream) {
     const Rows rows = make_rows(x, temperature);
+    // A gradient will read the rows again, the last ones first: as many as the memory-side cache has room for are left
+    // in it.
+    const double row = double(x.vocab) * (x.type == MAMW_F32 ? 4.0 : 2.0);
+    const uint32_t keep_from = stats ? uint32_t(fmax(0.0, rows.rows - kKeptBytes / row)) : uint32_t(rows.rows);
     return with_type(x.type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto n) {
@@ -276,7 +289,7 @@ int launch_logprobs(const mamw_rows& x, const mamw_per_row& tokens, int64_t igno
             return int(launch(K_OBJ_LOGPROBS, entropy ? 1 : 0, 0.0, row_bytes(x, false),
                               entropy ? logprobs_kernel<T, kN, true> : logprobs_kernel<T, kN, false>,
                               row_grid(rows.rows), dim3(kN), stream, rows, make_per_row(tokens), ignore,
-                              logprobs, entropy, stats, coef, ticket));
+                              logprobs, entropy, stats, coef, ticket, keep_from));
         };
         // By the vocabulary alone, so that a row's result does not depend on how many there are.
         const int64_t vecs = x.vocab / kVec<T>;
