@@ -457,7 +457,7 @@ struct HeldRow {
     __device__ __forceinline__ Stats stats(float c, Hold hold, Change change) {
         Stats st = no_stats();
         if constexpr (kRest) {
-            read_vecs<T, false, false, kThreads_>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
+            read_vecs<T, false, false, kThreads_, true>(st, vecs(), kVecs * kThreads_, span.vecs, c, change);
             load_held(row);  // never without a vector
         }
         // In groups, each as its loads arrive: the sum is taken below the thread's largest logit so far and moved when
