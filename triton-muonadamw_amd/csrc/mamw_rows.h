@@ -197,17 +197,21 @@ __device__ __forceinline__ Floats<N> block_sum(Floats<N> x, float* lds) {
 // 4096 x 128256 bf16).
 __device__ __forceinline__ float below(float x, float m, float c) { return (x - m) * c; }
 
-// A row as `vecs` vectors on 16-byte boundaries, from element `head` on, and `extra` single elements before and after
-// them.  Loads that straddle the boundary cost: 8192 x 50257 bf16 with its odd rows took 162 us to read, against 117
-// for as many bytes on the boundary.
+// A row as `vecs` vectors of 16 bytes from the first 128-byte boundary on, at element `head`, and `extra` single
+// elements before and after them, at most kExtra.  A wave's 64 vectors are whole lines of the cache then.  Loads that
+// straddle 16 bytes cost: 8192 x 50257 bf16 with its odd rows took 162 us to read, against 117 for as many bytes on the
+// boundary; stores that share lines, too (4096 x 50257 fp32 with its gradient: 232 us from the first 16-byte boundary,
+// 212 from the first of 64, 206 of 128, 207 of 256).
 struct Span {
     int head, vecs, extra;
 };
+constexpr uintptr_t kLine = 128;
+constexpr int kExtra = 63 + 7;
 
 template <typename T>
 __device__ __forceinline__ Span span_of(const T* row, int vocab) {
     Span s;
-    s.head = min(vocab, int((-reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)));
+    s.head = min(vocab, int((-reinterpret_cast<uintptr_t>(row) & (kLine - 1)) / sizeof(T)));
     s.vecs = (vocab - s.head) / kVec<T>;
     s.extra = s.head + (vocab - s.head) % kVec<T>;
     return s;
@@ -219,7 +223,8 @@ __device__ __forceinline__ int extra_element(const Span& s, int e) {
     return e < s.head ? e : e + s.vecs * kVec<T>;
 }
 
-// The thread of `threads` that writes element j, where vector n is thread n % threads' and single element e thread e's.
+// The thread of `threads` that writes element j, where vector n is thread n % threads' and single element e thread e's
+// (more than kExtra of them).
 template <typename T>
 __device__ __forceinline__ int owner_of(const Span& s, int j, int threads) {
     if (j < s.head) return j;
@@ -670,15 +675,16 @@ inline dim3 row_grid(int64_t rows) {
     return rows <= int64_t(most) ? dim3(unsigned(rows)) : dim3(most, unsigned((rows + most - 1) / most));
 }
 
-// Up to this many rows the last workgroup adds up the result; above, where the launch is long against another, a kernel
-// of its own does, and the workgroups need not wait for each other's memory.
-constexpr int64_t kTicketRows = 1024;
+// Up to this many workgroups the last one adds up the result, above a kernel of its own does.  The launch saved is 4 us on
+// the device and as many on the host; the ticket costs each workgroup a write-back of its L2 cache (64 rows: 6 us
+// instead of 5 and 4 for the other launch; 256 x 50257 fp32: 30 instead of 18 and 4; 1024: 124 instead of 67 and 4).
+constexpr int64_t kTickets = 64;
 
 // Where the rows' parts of `result` go; `launched`: the ticket is cleared by a launch before.
 inline Result make_result(const ObjectiveWorkspace& ws, char* base, int64_t rows, bool launched, float f, float* result) {
     Result out;
     out.parts = reinterpret_cast<float4*>(base + ws.partials_at);
-    out.ticket = launched && rows <= kTicketRows ? reinterpret_cast<uint32_t*>(base + ws.ticket_at) : nullptr;
+    out.ticket = launched && rows <= kTickets ? reinterpret_cast<uint32_t*>(base + ws.ticket_at) : nullptr;
     out.of = uint32_t(rows);
     out.result = result;
     out.f = f;

@@ -203,20 +203,24 @@ struct Marks {
     static constexpr int kWords = (kVecs + 3) / 4;  // of a thread
     static constexpr int kHeld = kThreads_ * kWords;
 
-    static __host__ __device__ constexpr int words(int vocab) { return kHeld + 1 + (kRest ? (vocab + 31) / 32 : 0); }
+    static constexpr int kSingles = (kExtra + 31) / 32;
+    static constexpr int kTable = kHeld + kSingles;  // where the bits of all elements begin
+
+    static __host__ __device__ constexpr int words(int vocab) { return kTable + (kRest ? (vocab + 31) / 32 : 0); }
 
     // Marks element j, if `wave` is the wave that holds it, or -1.
     static __device__ __forceinline__ void set(uint32_t* table, const Span& s, int j, int wave) {
         const int n = j < s.head ? -1 : (j - s.head) / kVec<T>;
         const bool is_single = n < 0 || n >= s.vecs;
-        if (wave >= 0 && wave != (is_single ? 0 : n % kThreads_ / 64)) return;
+        const int single = j < s.head ? j : j - s.vecs * kVec<T>;
+        if (wave >= 0 && wave != (is_single ? single / 64 : n % kThreads_ / 64)) return;
         if (is_single) {
-            atomicOr(&table[kHeld], 1u << (j < s.head ? j : j - s.vecs * kVec<T>));
+            atomicOr(&table[kHeld + single / 32], 1u << (single & 31));
         } else if (n < kVecs * kThreads_) {
             const int i = n / kThreads_, k = (j - s.head) % kVec<T>;
             atomicOr(&table[n % kThreads_ * kWords + i / 4], 1u << (i % 4 * 8 + k));
         } else {
-            atomicOr(&table[kHeld + 1 + (j >> 5)], 1u << (j & 31));
+            atomicOr(&table[kTable + (j >> 5)], 1u << (j & 31));
         }
     }
 
@@ -239,8 +243,8 @@ struct Marks {
     // The bits of vector n, not held: elements head + n kVec and on.
     static __device__ __forceinline__ uint32_t rest(const uint32_t* table, const Span& s, int n, int vocab) {
         const int j = s.head + n * kVec<T>, w = j >> 5;
-        uint32_t m = table[kHeld + 1 + w] >> (j & 31);
-        if ((j & 31) + kVec<T> > 32 && w + 1 < (vocab + 31) / 32) m |= table[kHeld + 2 + w] << (32 - (j & 31));
+        uint32_t m = table[kTable + w] >> (j & 31);
+        if ((j & 31) + kVec<T> > 32 && w + 1 < (vocab + 31) / 32) m |= table[kTable + 1 + w] << (32 - (j & 31));
         return m & ((1u << kVec<T>) - 1u);
     }
 };
@@ -297,7 +301,8 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
         const int wave = threadIdx.x / 64;
 #pragma unroll
         for (int i = 0; i < Mark::kWords; ++i) marked[int(threadIdx.x) * Mark::kWords + i] = 0;
-        if (threadIdx.x == 0) marked[Mark::kHeld] = 0;
+        // single element e is thread e's: two words of wave 0, one of wave 1
+        if (threadIdx.x % 32 == 0 && int(threadIdx.x) < 32 * Mark::kSingles) marked[Mark::kHeld + threadIdx.x / 32] = 0;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
     if constexpr (kTail) {
 #pragma unroll
         for (int i = 0; i < Mark::kWords; ++i) mine[i] = marked[int(threadIdx.x) * Mark::kWords + i];
-        if (held.has_single() && (marked[Mark::kHeld] >> threadIdx.x & 1u)) held.single_ = raw_nothing<T>();
+        if (held.has_single() && (marked[Mark::kHeld + threadIdx.x / 32] >> (threadIdx.x & 31) & 1u)) held.single_ = raw_nothing<T>();
     }
     auto hold = [&](vec_t& v, int i) {
         if constexpr (kTail) {

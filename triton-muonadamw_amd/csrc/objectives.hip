@@ -34,9 +34,10 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
         auto stats_of_row = [&](auto quick) {
             constexpr bool kQuick = decltype(quick)::value != 0;
             Stats st = no_stats();
-            if (int(threadIdx.x) < span.extra) {
-                st.m = widen(row[extra_element<T>(span, threadIdx.x)]);
-                add<kEntropy>(st, st.m, reference(st.m), x.c);
+            for (int e = threadIdx.x; e < span.extra; e += kThreads_) {
+                const float single = widen(row[extra_element<T>(span, e)]);
+                move_to<kEntropy>(st, fmaxf(st.m, single), x.c);
+                add<kEntropy>(st, single, reference(st.m), x.c);
             }
             if (kQuick && r >= keep_from)
                 read_vecs<T, kEntropy, kQuick, kThreads_, true>(st, row + span.head, 0, span.vecs, x.c, Unchanged());
@@ -396,12 +397,7 @@ extern "C" int mamw_preference_loss(const mamw_rows* logits, const mamw_preferen
                                     reinterpret_cast<float*>(ticket), int64_t(1)));
     if (st != MAMW_OK) return st;
     const int64_t pairs = p->sequences / 2;
-    Result out;
-    out.parts = reinterpret_cast<float4*>(base + ws.partials_at);
-    out.ticket = ticket;
-    out.of = uint32_t(pairs);
-    out.result = result;
-    out.f = 1.f / float(pairs);
+    const Result out = make_result(ws, base, pairs, true, 1.f / float(pairs), result);
     Preference d;
     d.tokens = make_per_row(p->tokens);
     d.ignore = p->ignore_index;
@@ -411,6 +407,8 @@ extern "C" int mamw_preference_loss(const mamw_rows* logits, const mamw_preferen
     d.smoothing = p->smoothing;
     d.kind = p->kind;
     d.length_average = p->length_average;
-    return int(launch(K_OBJ_PAIRS, 0, 0.0, 0.0, pairs_kernel, row_grid(pairs), dim3(kThreads), s, rows, d,
-                      static_cast<const float*>(row_logprobs), logprobs, rewards, out, coef));
+    if ((st = int(launch(K_OBJ_PAIRS, 0, 0.0, 0.0, pairs_kernel, row_grid(pairs), dim3(kThreads), s, rows, d,
+                         static_cast<const float*>(row_logprobs), logprobs, rewards, out, coef))) != 0)
+        return st;
+    return launch_result(out, s);
 }
