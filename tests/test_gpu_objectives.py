@@ -244,6 +244,36 @@ def test_inputs_changed_in_place_are_noticed(gpu):
         loss.backward()
 
 
+@pytest.mark.parametrize("which", ["logprobs", "policy", "preference", "distill"])
+def test_graphs_used_twice(gpu, which):
+    """Backward a second time without retain_graph is torch's error; a gradient with create_graph is the same, and
+    differentiating it is an error."""
+    x, tokens, old, adv, _ = policy_case(6, 103, "fp32", 9)
+    x.requires_grad_()
+    index = torch.arange(4, device="cuda").repeat(6, 1)
+    make = {"logprobs": lambda: token_logprobs(x, tokens).sum(),
+            "policy": lambda: policy_loss(x, tokens, old, adv).loss,
+            "preference": lambda: preference_loss(x.view(2, 3, -1), tokens.view(2, 3), None).loss,
+            "distill": lambda: distill_loss(x, torch.ones((6, 4), device="cuda"), index)}[which]
+    loss = make()
+    first, = torch.autograd.grad(loss, x)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(loss, x)
+    again, = torch.autograd.grad(make(), x, create_graph=True)
+    assert torch.equal(first, again)
+    with pytest.raises(RuntimeError, match="differentiated a second time"):
+        again.sum().backward()
+
+
+def test_only_one_output_used(gpu):
+    """Entropies alone in the loss, and a graph that reaches the logits through a view."""
+    x, tokens, _ = make(6, 103, "fp32", 9)
+    x.requires_grad_()
+    a, = torch.autograd.grad(token_logprobs(x.view(2, 3, -1), tokens.view(2, 3), entropy=True)[1].sum(), x)
+    _, _, egrad = ob.token_logprobs(f64(x), tokens.cpu().numpy(), dentropy=np.ones(6))
+    check_grad(a, egrad, 1e-5)
+
+
 # ---- preference_loss
 
 @pytest.mark.parametrize("dtype", list(DTYPES))

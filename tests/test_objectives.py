@@ -107,6 +107,14 @@ def test_refused(call, error, text):
         call()
 
 
+@pytest.mark.parametrize("fn", ALL)
+def test_forward_mode_is_refused(fn):
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        fn(fwd.make_dual(X, torch.ones_like(X)))
+
+
 # ---- the C ABI
 
 BASE = 1 << 40

@@ -6,6 +6,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -14,6 +15,8 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+
+#include <pybind11/pybind11.h>
 
 #include <mutex>
 
@@ -128,6 +131,7 @@ std::pair<Tensor, int64_t> sequences(const Tensor& offsets, const Tensor& logits
 
 // Last of the checks: the kernels run on ROCm devices only.
 void require_gpu(const Tensor& logits) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!logits._fw_grad(/*level=*/0).defined(), "the objectives have no forward-mode derivative");
     TORCH_CHECK(logits.is_cuda(), "logits is on ", logits.device(),
                 "; MuonAdamW's HIP kernels need tensors on a ROCm GPU (there is no CPU path)");
 }
@@ -152,6 +156,15 @@ SavedVariable keep(const Tensor& t) {
 
 // ---- the autograd graph
 
+// A gradient that was computed for a graph to be built of it (create_graph) cannot be differentiated again: who tries
+// gets an error, not zeros.
+Tensor once(const Tensor& grad) {
+    if (!at::GradMode::is_enabled()) return grad;
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "the objectives' gradients cannot be differentiated a second time", 1);
+    return (*error)({grad.detach().requires_grad_(true)})[0];
+}
+
 // A loss whose forward kernel writes the gradient as well, because a row's gradient needs nothing beyond that row.
 // backward hands it out; a gradient of the loss other than 1 has it computed again from the logits with that factor
 // (the device decides, so nothing waits), which rounds once and keeps float16 gradients of a scaled loss from
@@ -168,6 +181,10 @@ struct OnePass : Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> guard(lock);
         if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+        return {once(gradient(grads[0]))};
+    }
+
+    Tensor gradient(const Tensor& grad_output) {
         at::NoGradGuard no_grad;
         const Tensor x = logits.unpack();  // raises where it was released, or changed in place since
         for (auto& i : inputs) i.unpack();
@@ -176,9 +193,9 @@ struct OnePass : Node {
         grad = Tensor();
         const bool fresh = !out.defined();  // the graph was retained and the first one is someone else's now
         if (fresh) out = grad_like(x);
-        const Tensor scale = grads[0].to(at::kFloat);
+        const Tensor scale = grad_output.to(at::kFloat);
         check(again(ptr<float>(scale), !fresh, ptr(out), stream_of(x)), name().c_str());
-        return {out};
+        return out;
     }
 
     void release_variables() override {
@@ -219,6 +236,10 @@ struct FromStats : Node {
         const bool by_row = !coef.defined();
         const bool second = by_row && entropy.defined() && grads.size() > 1 && grads[1].defined();
         if (!task_should_compute_output(0) || !(grads[0].defined() || second)) return {Tensor()};
+        return {once(gradient(grads, by_row, second))};
+    }
+
+    Tensor gradient(const variable_list& grads, bool by_row, bool second) {
         at::NoGradGuard no_grad;
         const Tensor x = logits.unpack(), toks = tokens.unpack();
         const c10::DeviceGuard device(x.device());
@@ -241,7 +262,7 @@ struct FromStats : Node {
                                second ? &h : nullptr, ptr<float>(entropy), by_row ? nullptr : ptr<float>(first),
                                ptr(out), stream_of(x)),
               name().c_str());
-        return {out};
+        return out;
     }
 
     void release_variables() override {
@@ -325,6 +346,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const bool grad = wants_grad(logits);
     Tensor logprobs, entropy, stats;
     {
+        pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard device(logits.device());
         const auto shape = logits.sizes().slice(0, logits.dim() - 1);
@@ -356,6 +378,7 @@ Tensor with_node(const Tensor& logits, const std::shared_ptr<N>& node, const mam
                  std::initializer_list<Tensor> inputs, Fn forward) {
     Tensor loss, grad;
     {
+        pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
         if (node) grad = grad_like(logits);
         loss = forward(ptr(grad));
@@ -407,6 +430,7 @@ PyObject* policy_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     Tensor logprobs, kl, clipped, workspace;
     {
+        pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
         workspace = bytes(need, logits);
         logprobs = floats(logits.sizes().slice(0, logits.dim() - 1), logits);
@@ -461,6 +485,7 @@ PyObject* preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const bool grad = wants_grad(logits);
     Tensor loss, logprobs, rewards, stats, coef;
     {
+        pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard device(logits.device());
         const Tensor workspace = bytes(need, logits);
@@ -523,6 +548,7 @@ PyObject* distill_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     Tensor workspace;
     {
+        pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
         workspace = bytes(need, logits);
     }

@@ -174,15 +174,12 @@ def _build_layout(verbose: bool) -> None:
 
 
 def _build_objectives(verbose: bool) -> None:
-    """The objectives' torch calls, linked against the library beside them.  The
-    optimizer does not need them, so here, too, a failure is a warning; calling
-    an objective raises then (``_lib.objectives``)."""
+    """The objectives' torch calls, linked against the library beside them."""
     failed = _build_module("objectives_module.cpp", OBJECTIVES_PATH, verbose, f"-I{INCLUDE}", "-I/opt/rocm/include",
                            "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-lc10_hip", f"-L{PKG_DIR}", f"-l:{LIB_NAME}",
                            "-Wl,-rpath,$ORIGIN")
     if failed:
-        warnings.warn(f"triton_muon_adamw._objectives was not built: the objectives cannot be used.{failed}",
-                      RuntimeWarning, stacklevel=2)
+        raise RuntimeError(f"triton_muon_adamw._objectives was not built: the objectives cannot be used.{failed}")
 
 
 def build(verbose: bool = False) -> Path:
