@@ -224,7 +224,7 @@ __device__ __forceinline__ int extra_element(const Span& s, int e) {
 }
 
 // The thread of `threads` that writes element j, where vector n is thread n % threads' and single element e thread e's
-// (more than kExtra of them).
+// (there are more threads than kExtra).
 template <typename T>
 __device__ __forceinline__ int owner_of(const Span& s, int j, int threads) {
     if (j < s.head) return j;
@@ -261,11 +261,16 @@ __device__ __forceinline__ void zero_row(T* __restrict__ g, int vocab, int threa
     if (int(threadIdx.x) < s.extra) g[extra_element<T>(s, threadIdx.x)] = narrow<T>(0.f);
 }
 
-// The logit of the row's token: NaN where it is beyond the vocabulary.
+// The logit of the row's token, on its way.
 template <typename T>
-__device__ __forceinline__ float chosen(const T* x, int64_t token, int vocab) {
-    return token >= 0 && token < vocab ? widen(x[token]) : NAN;
-}
+struct Chosen {
+    bool beyond;  // the vocabulary
+    Raw<T> raw;
+
+    __device__ __forceinline__ Chosen(const T* row, int64_t token, int vocab)
+        : beyond(token < 0 || token >= vocab), raw(raw_at(row + (beyond ? 0 : token))) {}
+    __device__ __forceinline__ float value() const { return beyond ? NAN : raw.value(); }
+};
 
 // Running softmax statistics: the largest logit m so far, s = sum of 2^y and sy = sum of 2^y y (entropies) below it.
 struct Stats {
@@ -341,7 +346,9 @@ __device__ __forceinline__ bool quick_holds(const Stats& st) {
 // The statistics of vectors from + threadIdx.x, + kThreads_, ... below `to`; change(v, n) is applied to vector n.
 template <typename T, bool kEntropy, bool kQuick, int kThreads_, bool kKeep = false, typename Change>
 __device__ __forceinline__ void read_vecs(Stats& st, const void* vecs, int from, int to, float c, Change change) {
-    constexpr int kUnroll = 4;
+    // Two: more take the registers of waves that would hide the exponentials (8192 x 50257 bf16 with entropies: 93 us with
+    // four, 87 with three, 84 with two, 91 with one).
+    constexpr int kUnroll = 2;
     const int t = threadIdx.x;
     vec_t v[kUnroll];
     int n = from;
@@ -649,7 +656,7 @@ inline double row_bytes(const mamw_rows& x, bool grad) {
 
 // fn(workgroup size, vectors a thread, whether some are left) for rows of `vecs` vectors, held by one workgroup.
 // Each thread keeps one to sixteen: fewer threads of more would leave the reductions to fewer waves, and a row of 256
-// KiB is all the registers of a compute unit that its other values leave.  A longer row keeps 192 KiB and has the rest
+// KiB is all the registers of a compute unit that its other values leave.  A longer row keeps that much and has the rest
 // read twice.
 template <int kN>
 struct Int {
@@ -664,7 +671,7 @@ int with_held_row(int64_t vecs, Fn fn) {
     if (vecs <= 4096) return fn(Int<512>(), Int<8>(), Int<0>());
     if (vecs <= 8192) return fn(Int<512>(), Int<16>(), Int<0>());
     if (vecs <= 16384) return fn(Int<1024>(), Int<16>(), Int<0>());
-    return fn(Int<1024>(), Int<12>(), Int<1>());
+    return fn(Int<1024>(), Int<16>(), Int<1>());
 }
 
 // One workgroup a row.  Such workgroups come and go by themselves: a row's loads do not wait for the stores of the row

@@ -35,8 +35,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
         return;
     }
     const T* row = row_of<T>(x, at);
-    const bool beyond = token < 0 || token >= x.vocab;
-    const Raw<T> xt_ = raw_at(row + (beyond ? 0 : token));
+    const Chosen<T> chosen(row, token, x.vocab);
     const Counts counted(p.count, p.items, p.by_sequence);
     const float old = load_f32(p.old, at), adv = load_f32(p.advantages, at);
     const float ref = p.ref.data ? load_f32(p.ref, at) : 0.f;
@@ -45,7 +44,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
     const Stats wave = held.stats(x.c, Unchanged(), Unchanged());
     const Stats st = over_block<false, kThreads_>(wave, x.c, lds);
     const float w = 1.f / (length * counted.all());
-    const float xt = beyond ? NAN : xt_.value();
+    const float xt = chosen.value();
     const float lp = (xt - st.m) * x.inv_t - logf(st.s);
     const float ratio = expf(lp - old);
     const float bound = fminf(fmaxf(ratio, 1.f - p.low), 1.f + p.high);
@@ -60,10 +59,10 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
     }
     if (logprobs && threadIdx.x == 0) logprobs[r] = lp;
     if (g) {
-        const float a = beyond ? NAN : f * p.scale * w * slope * x.inv_t, b = -a / st.s;
+        const float a = chosen.beyond ? NAN : f * p.scale * w * slope * x.inv_t, b = -a / st.s;
         held.write(g, b, st.m, x.c, Unchanged());
         // by the thread that wrote the element: its writes stay in order
-        if (!beyond && int(threadIdx.x) == owner_of<T>(held.span, int(token), kThreads_))
+        if (!chosen.beyond && int(threadIdx.x) == owner_of<T>(held.span, int(token), kThreads_))
             g[token] = narrow<T>(a + b * __builtin_amdgcn_exp2f(below(xt, st.m, x.c)));
     }
     put_part(out, r, w * p.scale * loss, w * kl, clipped ? w : 0.f);

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
     if (ticket && r == 0 && threadIdx.x == 0) *ticket = 0;
     if (token != ignore) {
         const T* row = row_of<T>(x, at);
-        const float xt = chosen(row, token, x.vocab);
+        const Chosen<T> chosen(row, token, x.vocab);
         const Span span = span_of(row, x.vocab);
         auto stats_of_row = [&](auto quick) {
             constexpr bool kQuick = decltype(quick)::value != 0;
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
         Stats st = stats_of_row(Int<1>());
         if (!quick_holds<kEntropy>(st)) st = stats_of_row(Int<0>());
         const float log_s = logf(st.s);
-        lp = (xt - st.m) * x.inv_t - log_s;
+        lp = (chosen.value() - st.m) * x.inv_t - log_s;
         h = log_s - kLn2 * st.sy / st.s;
         if (stats && threadIdx.x == 0) {
             stats[2 * int64_t(r)] = st.m;
