@@ -197,6 +197,44 @@ def test_policy_rows_outside_sequences(gpu):
     check_policy(x, inside, old, adv, ref, out, x.grad, kl_coef=0.2, sequences=[(2, 5), (5, 9)])
 
 
+@pytest.mark.parametrize("rows", [3, 5000])
+def test_no_sequences(gpu, rows):
+    """Offsets of one place: no sequence, so nothing counts."""
+    x, tokens, old, adv, _ = policy_case(rows, 9, "fp32", 5, ignored=0.0)
+    x.requires_grad_()
+    out = policy_loss(x, tokens, old, adv, average="sequence", offsets=torch.zeros(1, dtype=torch.int64, device="cuda"))
+    out.loss.backward()
+    assert out.loss == 0 and out.clipped == 0 and not x.grad.any()
+
+
+def test_many_rows(gpu):
+    """More rows than one workgroup adds up, and more than fit the first dimension of a launch's grid."""
+    rows, vocab = 70001, 5
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = normal((rows, vocab), 2.0, gen)
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=gen)
+    old, adv = normal(rows, 0.3, gen) - 1.6, normal(rows, 1.0, gen) + 0.5
+    y = x.clone().requires_grad_()
+    out = policy_loss(y, tokens, old, adv)
+    out.loss.backward()
+    logq = torch.log_softmax(x.double(), -1)
+    lp = logq.gather(1, tokens[:, None])[:, 0]
+    ratio, a = (lp - old.double()).exp(), adv.double()
+    bound = ratio.clamp(0.8, 1.2)
+    size = (ratio.abs() * a.abs()).mean().item()
+    assert abs(out.loss.item() + torch.minimum(ratio * a, bound * a).mean().item()) <= 64 * U * size
+    slope = torch.where(bound * a < ratio * a, 0.0, -a * ratio) / rows
+    g = (torch.nn.functional.one_hot(tokens, vocab) - logq.exp()) * slope[:, None]
+    assert ((y.grad.double() - g).abs() <= 64 * U * (ratio * a.abs())[:, None] / rows).all()
+    assert (token_logprobs(x, tokens).double() - lp).abs().max() <= 64 * U
+    index = tokens[:, None]
+    assert distill_loss(x, torch.zeros_like(index, dtype=torch.float32), index).item() == pytest.approx(
+        -lp.mean().item(), rel=1e-6)
+    half = preference_loss(x[:70000].view(1000, 70, 5), tokens[:70000].view(1000, 70), None)
+    s = lp[:70000].view(2, 500, 70).sum(-1)
+    assert half.loss.item() == pytest.approx(-torch.nn.functional.logsigmoid(0.1 * (s[0] - s[1])).mean().item(), rel=1e-5)
+
+
 def test_offsets_that_hold_anything_stay_inside(gpu):
     """Offsets beyond the rows are cut to them; nothing is read outside."""
     x, tokens, old, adv, _ = policy_case(12, 65, "fp32", 5, ignored=0.0)

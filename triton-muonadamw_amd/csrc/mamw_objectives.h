@@ -11,6 +11,8 @@ namespace mamw {
 
 // Rows whose tokens one block of the counting kernel looks at where sequences do not matter.
 constexpr int kCountRows = 1024;
+// Workgroups of the kernel that adds up the rows' parts of a result, at most.
+constexpr int kResultBlocks = 64;
 // Rows of teacher's entries that one workgroup prepares.
 constexpr int kTeacherRows = 16;
 // Bits of the table of a teacher's indices in rows that are not held whole (128 KiB of LDS at most).
@@ -20,7 +22,7 @@ constexpr int64_t kMaxTailVocab = int64_t(1) << 20;
 // row's sequence (policy, by sequence) or its teacher's entries, the rows' parts of the result.
 struct ObjectiveWorkspace {
     int64_t items;      // counts
-    size_t ticket_at;   // bytes from the start
+    size_t ticket_at;   // bytes from the start; kResultBlocks parts of 16 bytes behind 256
     size_t lengths_at;
     size_t partials_at;
     size_t bytes;

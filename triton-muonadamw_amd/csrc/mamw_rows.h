@@ -654,22 +654,35 @@ inline double row_bytes(const mamw_rows& x, bool grad) {
     return double(x.outer * x.inner) * double(x.vocab) * (x.type == MAMW_F32 ? 4.0 : 2.0) * (grad ? 2.0 : 1.0);
 }
 
-// fn(workgroup size, vectors a thread, whether some are left) for rows of `vecs` vectors, held by one workgroup.
-// Each thread keeps one to sixteen: fewer threads of more would leave the reductions to fewer waves, and a row of 256
-// KiB is all the registers of a compute unit that its other values leave.  A longer row keeps that much and has the rest
-// read twice.
+// fn(workgroup size, vectors a thread, whether some are left) for rows of `vecs` vectors, held by one workgroup.  Four
+// vectors a thread, as long as there are threads for it, measured best; halves and doubles of it, us for 1.6 GB:
+//     4000 bf16 (500 vectors)     128 x 4: 151   256 x 2: 158   512 x 1: 271
+//     8000 (1000)                 128 x 8: 167   256 x 4: 159   512 x 2: 175
+//     16000 (2000)                256 x 8: 161   512 x 4: 152  1024 x 2: 181
+//     32000 (4000)               256 x 16: 157   512 x 8: 155  1024 x 4: 145
+//     50257 (6282)               512 x 16: 248  1024 x 8: 244
+// That is for a kernel of few registers: two workgroups of 1024 share a compute unit if a thread takes 64 at most.  One
+// of more has workgroups of 512 for the long rows (distillation with a rest: 32000 bf16 152 with 512 x 8, 159 with
+// 1024 x 4; 50257 266 with 512 x 16, 322 with 1024 x 8).
+// A row of 256 KiB is all the registers of a compute unit that its other values leave.  A longer row keeps that much and
+// has the rest read twice.
 template <int kN>
 struct Int {
     static constexpr int value = kN;
 };
-template <typename Fn>
+template <bool kMoreRegisters, typename Fn>
 int with_held_row(int64_t vecs, Fn fn) {
-    if (vecs <= 256) return fn(Int<256>(), Int<1>(), Int<0>());
-    if (vecs <= 512) return fn(Int<256>(), Int<2>(), Int<0>());
+    if (vecs <= 256) return fn(Int<128>(), Int<2>(), Int<0>());
+    if (vecs <= 512) return fn(Int<128>(), Int<4>(), Int<0>());
     if (vecs <= 1024) return fn(Int<256>(), Int<4>(), Int<0>());
-    if (vecs <= 2048) return fn(Int<256>(), Int<8>(), Int<0>());
-    if (vecs <= 4096) return fn(Int<512>(), Int<8>(), Int<0>());
-    if (vecs <= 8192) return fn(Int<512>(), Int<16>(), Int<0>());
+    if (vecs <= 2048) return fn(Int<512>(), Int<4>(), Int<0>());
+    if constexpr (kMoreRegisters) {
+        if (vecs <= 4096) return fn(Int<512>(), Int<8>(), Int<0>());
+        if (vecs <= 8192) return fn(Int<512>(), Int<16>(), Int<0>());
+    } else {
+        if (vecs <= 4096) return fn(Int<1024>(), Int<4>(), Int<0>());
+        if (vecs <= 8192) return fn(Int<1024>(), Int<8>(), Int<0>());
+    }
     if (vecs <= 16384) return fn(Int<1024>(), Int<16>(), Int<0>());
     return fn(Int<1024>(), Int<16>(), Int<1>());
 }
@@ -702,6 +715,6 @@ inline Result make_result(const ObjectiveWorkspace& ws, char* base, int64_t rows
 int launch_count(const Rows& rows, const PerRow& tokens, int64_t ignore, const PerRow& mask, const Sequences& seqs,
                  const ObjectiveWorkspace& ws, bool by_sequence, char* base, hipStream_t stream);
 // result_kernel, where the workgroups had no ticket.
-int launch_result(const Result& out, hipStream_t stream);
+int launch_result(const Result& out, const ObjectiveWorkspace& ws, char* base, hipStream_t stream);
 
 }  // namespace mamw

@@ -442,7 +442,7 @@ int launch_distill(const mamw_rows& x, const mamw_distill& p, const ObjectiveWor
     const bool tail = p.teacher_lse.data != nullptr;
     return with_type(x.type, [&](auto t) {
         using T = decltype(t);
-        return with_held_row(x.vocab / kVec<T>, [&](auto n, auto v, auto rest) {
+        return with_held_row<true>(x.vocab / kVec<T>, [&](auto n, auto v, auto rest) {
             constexpr int kN = decltype(n)::value, kV = decltype(v)::value;
             constexpr bool kRest = decltype(rest)::value != 0;
             const size_t lds = tail ? size_t(Marks<T, kN, kV, kRest>::words(int(x.vocab))) * 4 : 0;
@@ -481,7 +481,7 @@ extern "C" int mamw_distill_loss(const mamw_rows* logits, const mamw_distill* p,
     if ((st = launch_teacher(*logits, *p, ws, w, s)) != MAMW_OK) return st;
     const Result out = make_result(ws, base, rows, rows > 0, p->scale * p->temperature * p->temperature, result);
     if ((st = launch_distill(*logits, *p, ws, w, out, nullptr, 0, grad, s)) != MAMW_OK) return st;
-    return launch_result(out, s);
+    return launch_result(out, ws, base, s);
 }
 
 extern "C" int mamw_distill_grad(const mamw_rows* logits, const mamw_distill* p, const float* scale, int unless_one,

@@ -88,7 +88,7 @@ int launch_policy(const mamw_rows& x, const mamw_policy& p, const ObjectiveWorks
     d.lengths = reinterpret_cast<const float*>(base + ws.lengths_at);
     return with_type(x.type, [&](auto t) {
         using T = decltype(t);
-        return with_held_row(x.vocab / kVec<T>, [&](auto n, auto v, auto rest) {
+        return with_held_row<false>(x.vocab / kVec<T>, [&](auto n, auto v, auto rest) {
             constexpr int kN = decltype(n)::value;
             return int(launch(K_OBJ_POLICY, kN, 0.0, row_bytes(x, grad != nullptr),
                               policy_kernel<T, kN, decltype(v)::value, decltype(rest)::value != 0>,
@@ -125,9 +125,9 @@ extern "C" int mamw_policy_loss(const mamw_rows* logits, const mamw_policy* p, f
     if ((st = launch_count(rows, make_per_row(p->tokens), p->ignore_index, none, {p->offsets, p->sequences}, ws,
                            p->by_sequence, base, s)) != MAMW_OK)
         return st;
-    const Result out = make_result(ws, base, rows.rows, ws.items > 0 && rows.rows > 0, 1.f, result);
+    const Result out = make_result(ws, base, rows.rows, rows.rows > 0, 1.f, result);
     if ((st = launch_policy(*logits, *p, ws, logprobs, out, nullptr, 0, grad, base, s)) != MAMW_OK) return st;
-    return launch_result(out, s);
+    return launch_result(out, ws, base, s);
 }
 
 extern "C" int mamw_policy_grad(const mamw_rows* logits, const mamw_policy* p, const float* scale, int unless_one,

@@ -29,7 +29,7 @@ ObjectiveWorkspace objective_workspace(int64_t items, int64_t lengths, int64_t p
     ObjectiveWorkspace w;
     w.items = items;
     w.ticket_at = round_up(size_t(items) * 4);
-    w.lengths_at = w.ticket_at + 256;
+    w.lengths_at = w.ticket_at + 256 + round_up(kResultBlocks * 16);
     w.partials_at = w.lengths_at + round_up(size_t(lengths) * 4);
     w.bytes = w.partials_at + round_up(size_t(partials) * 4);
     return w;
