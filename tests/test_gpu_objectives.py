@@ -185,6 +185,23 @@ def test_policy_sequences(gpu, packed, average):
                  sequences=seqs if average == "sequence" else None)
 
 
+@pytest.mark.parametrize("packed", [False, True])
+def test_policy_many_sequences(gpu, packed):
+    """More sequences than are counted one by one; every third without a token that counts, packed ones also empty."""
+    x, tokens, old, adv, ref = policy_case(3 * 131, 17, "fp32", 8)
+    tokens.view(131, 3)[::3] = -100
+    bounds = [min(2 * i, 393) for i in range(1 + 210)] if packed else list(range(0, 394, 3))
+    kw = {}
+    if packed:
+        kw["offsets"] = torch.tensor(bounds, device="cuda")
+    else:
+        x, tokens, old, adv, ref = (t.view(131, 3, *t.shape[1:]) for t in (x, tokens, old, adv, ref))
+    x.requires_grad_()
+    out = policy_loss(x, tokens, old, adv, ref_logprobs=ref, kl_coef=0.2, average="sequence", **kw)
+    out.loss.backward()
+    check_policy(x, tokens, old, adv, ref, out, x.grad, kl_coef=0.2, sequences=list(zip(bounds, bounds[1:])))
+
+
 def test_policy_rows_outside_sequences(gpu):
     """Rows before the first offset and after the last do not count with average="sequence"."""
     x, tokens, old, adv, ref = policy_case(12, 65, "fp32", 5, ignored=0.0)

@@ -193,15 +193,15 @@ __device__ __forceinline__ Floats<N> block_sum(Floats<N> x, float* lds) {
 // ---- a row
 
 // y_j = log2 of exp((x_j - m) / T).  The difference first: logits and masks may be the type's lowest value, whose
-// product with log2(e) / T overflows (the fused form, one operation less, is no faster: 399 against 401 us for
-// 4096 x 128256 bf16).
+// product with log2(e) / T overflows.  (The fused form, one operation less, is as fast where memory is the bound: 590
+// against 586 us for a policy loss over 8192 x 128256 bf16; 319 against 325 for a distillation over 4096 of them.)
 __device__ __forceinline__ float below(float x, float m, float c) { return (x - m) * c; }
 
 // A row as `vecs` vectors of 16 bytes from the first 128-byte boundary on, at element `head`, and `extra` single
 // elements before and after them, at most kExtra.  A wave's 64 vectors are whole lines of the cache then.  Loads that
 // straddle 16 bytes cost: 8192 x 50257 bf16 with its odd rows took 162 us to read, against 117 for as many bytes on the
-// boundary; stores that share lines, too (4096 x 50257 fp32 with its gradient: 232 us from the first 16-byte boundary,
-// 212 from the first of 64, 206 of 128, 207 of 256).
+// boundary; stores that share lines, too (4096 x 50257 fp32 with its gradient: 234 us from the first 16-byte boundary,
+// 212 from the first of 64, 207 of 128, 207 of 256).
 struct Span {
     int head, vecs, extra;
 };
@@ -232,8 +232,8 @@ __device__ __forceinline__ int owner_of(const Span& s, int j, int threads) {
     return n < s.vecs ? n % threads : j - s.vecs * kVec<T>;
 }
 
-// Rows pass through once: kept out of the caches' way (4096 x 128256 bf16, read and written: 399 us without, 375
-// with).
+// Rows pass through once: kept out of the caches' way (8192 x 128256 bf16 and their gradient: 620 us with ordinary
+// loads and stores, 586 with these; the log-probabilities of 8192 x 50257 bf16: 94 and 83).
 //
 // Vector `thread` of those from `first` on, with `first` the same for the whole workgroup: scalar address and 32-bit
 // offset, no registers for sixteen 64-bit addresses.
@@ -558,17 +558,15 @@ struct Unchanged {
 struct Counts {
     const int32_t* count;
     int64_t items;
-    bool by_sequence;
     int32_t first;
 
-    __device__ __forceinline__ Counts(const int32_t* count_, int64_t items_, bool by_sequence_)
-        : count(count_), items(items_), by_sequence(by_sequence_),
+    __device__ __forceinline__ Counts(const int32_t* count_, int64_t items_)
+        : count(count_), items(items_),
           first(count_[max(min(int64_t(threadIdx.x % 64), items_ - 1), int64_t(0))]) {}
-    __device__ __forceinline__ float one(int32_t n) const { return by_sequence ? float(n > 0) : float(n); }
     __device__ __forceinline__ float all() const {
         const int lane = threadIdx.x % 64;
-        float n = lane < items ? one(first) : 0.f;
-        for (int64_t i = 64 + lane; i < items; i += 64) n += one(count[i]);
+        float n = lane < items ? float(first) : 0.f;
+        for (int64_t i = 64 + lane; i < items; i += 64) n += float(count[i]);
         return fmaxf(wave_sum(n), 1.f);
     }
 };

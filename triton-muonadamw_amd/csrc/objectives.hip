@@ -13,6 +13,11 @@ namespace {
 
 // ---- token_logprobs
 
+// log q_t = (x_t - m) / T - log s and H = log s - sum 2^y y ln2 / s, with m the largest logit and s the sum of
+// exp((x - m) / T), both kept as the row goes by: a thread moves its sums when its largest logit grows, so that one read
+// is enough.  Bound by that read and, nearly as much, by eleven operations an element with entropies (VALU busy 0.9 of
+// the time): 5417 of 8192 rows of 50257 bf16 that count, 545 MB, in 83 us, 6.5 TB/s (a kernel that only reads: 7.0); the
+// statistics of 5101 of 6000, without entropies, in 87.
 template <typename T, int kThreads_, bool kEntropy>
 __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow tokens, int64_t ignore,
                                                              float* __restrict__ logprobs,
@@ -66,7 +71,11 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
 // A workgroup takes kGradVecs vectors of one row: it waits for nothing, so short-lived ones in great number come
 // nearest to a copy (6000 x 50257 bf16: 224 us with eight vectors a thread, 209 with four, 198 with two, 204 with
 // one).  Rows are taken from the last: those the statistics were taken of last are still in the memory-side cache of 256
-// MB (198 -> 183 us).
+// MB (198 -> 183 us; 176 with rows from the 128-byte boundary on).
+//
+// g_j = (c / T) ([j = t] - q_j) - (h / T) q_j (log q_j + H), with c and h the factors of the row's log-probability and
+// entropy.  Bound by memory: 513 MB read and 603 written in 176 us, 6.3 TB/s; 4096 x 128256 bf16, 630 and 1051 MB, in
+// 276, 6.1 TB/s (a copy: 6.06).
 constexpr int kGradUnroll = 2;
 constexpr int kGradVecs = kThreads * kGradUnroll;
 // Logits that the statistics leave there.  More than it holds, since of rows that do not count nothing is read; all of
@@ -155,8 +164,9 @@ __device__ __forceinline__ bool counts(const Rows& x, const PerRow& tokens, int6
     return load_mask(mask, at);
 }
 
-// counts[i]: rows that count of sequence i, and in lengths[] for each row of the sequence; or, with no sequences
-// (lengths NULL), of the kCountRows rows from i kCountRows on.
+// count[i]: of the kCountRows rows from i kCountRows on, how many count; or, with sequences (lengths not NULL), whether
+// any does of sequence i, and in lengths[] how many for each row of the sequence.
+// A few bytes a row: 4 us, a launch's latency and no more.
 __global__ __launch_bounds__(kThreads) void count_kernel(Rows x, PerRow tokens, int64_t ignore, PerRow mask,
                                                          Sequences seqs, uint32_t items, int32_t* __restrict__ count,
                                                          float* __restrict__ lengths,
@@ -170,10 +180,42 @@ __global__ __launch_bounds__(kThreads) void count_kernel(Rows x, PerRow tokens, 
     for (int64_t r = from + threadIdx.x; r < to; r += kThreads) n += counts(x, tokens, ignore, mask, uint32_t(r));
     // below 2^24 a thread; exact as floats where the sum is, too, else the weight's last bit
     const float all = block_sum(Floats<1>{{float(n)}}, lds).v[0];
-    if (threadIdx.x == 0) count[item] = int32_t(all);
+    if (threadIdx.x == 0) count[item] = lengths ? all > 0.f : int32_t(all);
     if (item == 0 && threadIdx.x == 0) *ticket = 0;
     if (lengths)
         for (int64_t r = from + threadIdx.x; r < to; r += kThreads) lengths[r] = all;
+}
+
+// The same for more than kCountGroups sequences: count[i] is how many of the i-th kCountGroups-th part of them have a row
+// that counts.  A wave takes a sequence.
+constexpr int kGroupThreads = 1024;
+__global__ __launch_bounds__(kGroupThreads) void count_groups_kernel(Rows x, PerRow tokens, int64_t ignore, PerRow mask,
+                                                                     Sequences seqs, int32_t* __restrict__ count,
+                                                                     float* __restrict__ lengths,
+                                                                     uint32_t* __restrict__ ticket) {
+    constexpr int kGroupWaves = kGroupThreads / 64;
+    __shared__ int with_any[kGroupWaves];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int64_t each = (seqs.count + kCountGroups - 1) / kCountGroups;
+    const int64_t first = blockIdx.x * each, end = min(first + each, seqs.count);
+    int some = 0;
+    for (int64_t i = first + wave; i < end; i += kGroupWaves) {
+        int64_t from, to;
+        sequence_rows(seqs, x, i, &from, &to);
+        int n = 0;
+        for (int64_t r = from + lane; r < to; r += 64) n += counts(x, tokens, ignore, mask, uint32_t(r));
+        const float all = wave_sum(float(n));
+        some += all > 0.f;
+        for (int64_t r = from + lane; r < to; r += 64) lengths[r] = all;
+    }
+    if (lane == 0) with_any[wave] = some;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int all = 0;
+        for (int w = 0; w < kGroupWaves; ++w) all += with_any[w];
+        count[blockIdx.x] = all;
+        if (blockIdx.x == 0) *ticket = 0;
+    }
 }
 
 __global__ __launch_bounds__(kThreads) void zero_kernel(float* __restrict__ x, int64_t n) {
@@ -182,7 +224,7 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(float* __restrict__ x, i
 }
 
 // The sums of the rows' parts, always in the same order: of kResultRows a workgroup, and of the workgroups' by the last of
-// them (one workgroup alone took 21 us for 65536 rows).
+// them (65536 rows: 5 us; one workgroup alone took 21).
 constexpr int kResultThreads = 1024;
 constexpr int kResultRows = 4096;
 __global__ __launch_bounds__(kResultThreads) void result_kernel(const float4* __restrict__ parts, uint32_t rows,
@@ -232,7 +274,7 @@ __device__ __forceinline__ double block_sum64(double x, double* lds) {
 
 // One workgroup a pair: the sums over both sequences, the pair's loss and the rows' coefficients.  The sums are of a
 // thousand log-probabilities, and what counts is how little they differ from a reference's: in 64 bits, as is the
-// margin.
+// margin.  Latency alone: a sequence's offsets, then its rows' tokens and log-probabilities (8 pairs, 6000 rows: 8 us).
 __global__ __launch_bounds__(kThreads) void pairs_kernel(Rows x, Preference p, const float* __restrict__ row_logprobs,
                                                          float* __restrict__ logprobs, float* __restrict__ rewards,
                                                          Result out, float* __restrict__ coef) {
@@ -322,6 +364,10 @@ int launch_count(const Rows& rows, const PerRow& tokens, int64_t ignore, const P
     if (ws.items == 0)
         return int(launch(K_OBJ_COUNT, 1, 0.0, 0.0, zero_kernel, dim3(1), dim3(kThreads), stream,
                           reinterpret_cast<float*>(ticket), int64_t(1)));
+    if (by_sequence && seqs.count > kCountGroups)
+        return int(launch(K_OBJ_COUNT, 2, 0.0, 0.0, count_groups_kernel, dim3(kCountGroups), dim3(kGroupThreads), stream, rows,
+                          tokens, ignore, mask, seqs, reinterpret_cast<int32_t*>(base),
+                          reinterpret_cast<float*>(base + ws.lengths_at), ticket));
     return int(launch(K_OBJ_COUNT, 0, 0.0, 0.0, count_kernel, row_grid(ws.items), dim3(kThreads), stream, rows,
                       tokens, ignore, mask, seqs, uint32_t(ws.items), reinterpret_cast<int32_t*>(base),
                       by_sequence ? reinterpret_cast<float*>(base + ws.lengths_at) : static_cast<float*>(nullptr),

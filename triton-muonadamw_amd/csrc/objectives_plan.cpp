@@ -101,7 +101,7 @@ int check_policy(const mamw_rows* x, const mamw_policy* p, const void* grad, Obj
     if ((st = check_temperature(p->temperature)) != MAMW_OK) return st;
     if (!(p->clip_low >= 0.f) || !(p->clip_high >= 0.f) || !isfinite(p->kl_coef) || !isfinite(p->scale))
         return MAMW_ERR_HYPER;
-    *ws = p->by_sequence ? objective_workspace(p->sequences, rows, 4 * rows)
+    *ws = p->by_sequence ? objective_workspace(p->sequences < kCountGroups ? p->sequences : kCountGroups, rows, 4 * rows)
                          : objective_workspace(count_items(rows), 0, 4 * rows);
     return MAMW_OK;
 }
@@ -142,7 +142,7 @@ int check_distill(const mamw_rows* x, const mamw_distill* p, const void* grad, O
     if (!isfinite(p->scale)) return MAMW_ERR_HYPER;
     if (p->teacher_lse.data && x->vocab > kMaxTailVocab) return MAMW_ERR_SHAPE;
     // Each row's entries (index, probability), its part of the result and what there is to know of its teacher.
-    *ws = objective_workspace((rows + kTeacherRows - 1) / kTeacherRows, 2 * rows * p->k, 8 * rows);
+    *ws = objective_workspace(count_items(rows), 2 * rows * p->k, 8 * rows);
     return MAMW_OK;
 }
 
