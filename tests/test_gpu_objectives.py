@@ -704,6 +704,43 @@ def test_nothing_counts(gpu):
     assert loss == 0 and not grad.any()
 
 
+def test_entropies_changed_in_place_raise(gpu):
+    x, tokens, _ = make(4, 65, "fp32", 0)
+    x.requires_grad_()
+    lp, ent = token_logprobs(x, tokens, entropy=True)
+    ent.mul_(0.5)
+    with pytest.raises(RuntimeError, match="inplace"):
+        ent.sum().backward()
+    lp, ent = token_logprobs(x, tokens, entropy=True)
+    (lp.sum() + (0.5 * ent).sum()).backward()
+    assert x.grad.isfinite().all()
+
+
+@pytest.mark.parametrize("which", ["logits", "shape", "tokens", "old"])
+def test_inputs_given_other_memory_raise(gpu, which):
+    """t.data = ... is seen by no version counter; backward reads by address."""
+    x, tokens, old, adv, _ = policy_case(4, 65, "fp32", 0, ignored=0.0)
+    leaf = x.clone().requires_grad_()
+    for loss in (lambda y: policy_loss(y, tokens, old, adv).loss, lambda y: token_logprobs(y, tokens).sum()):
+        if which == "old" and loss(leaf).grad_fn.name() != "PolicyLossBackward":
+            continue
+        y = leaf * 1.0
+        out = loss(y)
+        kept = tokens.data, old.data
+        if which == "logits":
+            y.data = torch.zeros_like(y)
+        elif which == "shape":
+            y.data = y.data[:2]
+        elif which == "tokens":
+            tokens.data = tokens.clone()
+        else:
+            old.data = old.clone()
+        with pytest.raises(RuntimeError, match="after the forward pass"):
+            out.backward()
+        tokens.data, old.data = kept
+        loss(leaf * 1.0).backward()
+
+
 @pytest.mark.parametrize("shape", [(0, 9), (0, 3, 9), (2, 0, 9)])
 def test_no_rows(gpu, shape):
     x = torch.zeros(shape, device="cuda", requires_grad=True)

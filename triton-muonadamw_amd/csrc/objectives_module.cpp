@@ -149,10 +149,35 @@ Tensor bytes(size_t n, const Tensor& like) {
     return at::empty({int64_t(n < 256 ? 256 : n)}, like.options().dtype(at::kByte));
 }
 
-// What an operator keeps of an input is its value: no gradient flows there.
-SavedVariable keep(const Tensor& t) {
-    return t.defined() ? SavedVariable(t.requires_grad() ? t.detach() : t, false) : SavedVariable();
-}
+// A tensor that backward reads by the address it had in the forward pass.  Its memory stays, and who has put other
+// memory under it meanwhile (t.data = ..., which no version counter sees) gets an error.
+struct Kept {
+    SavedVariable saved;
+    c10::Storage storage;
+    const void* data = nullptr;
+
+    Kept() = default;
+    // Of `logits` a gradient is wanted; what is kept of other inputs is their value.
+    Kept(const Tensor& t, bool logits = false)
+        : saved(!logits && t.requires_grad() ? t.detach() : t, false), storage(t.storage()), data(t.const_data_ptr()) {}
+
+    Tensor unpack() const {
+        Tensor t = saved.unpack();  // raises where it was released, or changed in place since
+        TORCH_CHECK(t.const_data_ptr() == data,
+                    "a tensor that the gradient needs was given other memory after the forward pass");
+        return t;
+    }
+    Tensor unpack(const mamw_rows& rows) const {
+        Tensor x = unpack();
+        TORCH_CHECK(x.dim() >= 1 && x.size(-1) == rows.vocab && x.numel() == rows.outer * rows.inner * rows.vocab,
+                    "logits changed their shape after the forward pass (now ", x.sizes(), ")");
+        return x;
+    }
+    void reset() {
+        saved.reset_data();
+        storage = c10::Storage();
+    }
+};
 
 // ---- the autograd graph
 
@@ -171,8 +196,8 @@ Tensor once(const Tensor& grad) {
 // vanishing first.
 struct OnePass : Node {
     std::mutex lock;
-    SavedVariable logits;
-    std::vector<SavedVariable> inputs;  // what the description points to
+    Kept logits;
+    std::vector<Kept> inputs;  // what the description points to
     mamw_rows rows;
     Tensor grad, workspace;
 
@@ -186,7 +211,7 @@ struct OnePass : Node {
 
     Tensor gradient(const Tensor& grad_output) {
         at::NoGradGuard no_grad;
-        const Tensor x = logits.unpack();  // raises where it was released, or changed in place since
+        const Tensor x = logits.unpack(rows);
         for (auto& i : inputs) i.unpack();
         const c10::DeviceGuard device(x.device());
         Tensor out = std::move(grad);
@@ -200,8 +225,8 @@ struct OnePass : Node {
 
     void release_variables() override {
         std::lock_guard<std::mutex> guard(lock);
-        logits.reset_data();
-        for (auto& i : inputs) i.reset_data();
+        logits.reset();
+        for (auto& i : inputs) i.reset();
         grad = workspace = Tensor();
     }
 };
@@ -226,24 +251,24 @@ struct DistillLossBackward : OnePass {
 // each row, and of the preference loss, with one for the loss and the rows' coefficients.
 struct FromStats : Node {
     std::mutex lock;
-    SavedVariable logits, tokens;
-    Tensor stats, coef, entropy;  // coef: the preference loss's
+    Kept logits, tokens, entropy;
+    mamw_rows rows;
+    Tensor stats, coef;  // coef: the preference loss's
     double temperature;
     int64_t ignore_index;
 
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> guard(lock);
         const bool by_row = !coef.defined();
-        const bool second = by_row && entropy.defined() && grads.size() > 1 && grads[1].defined();
+        const bool second = by_row && grads.size() > 1 && grads[1].defined();
         if (!task_should_compute_output(0) || !(grads[0].defined() || second)) return {Tensor()};
         return {once(gradient(grads, by_row, second))};
     }
 
     Tensor gradient(const variable_list& grads, bool by_row, bool second) {
         at::NoGradGuard no_grad;
-        const Tensor x = logits.unpack(), toks = tokens.unpack();
+        const Tensor x = logits.unpack(rows), toks = tokens.unpack(), h_out = second ? entropy.unpack() : Tensor();
         const c10::DeviceGuard device(x.device());
-        const mamw_rows rows = rows_of(x);
         const mamw_per_row at = per_row(toks, "tokens", x, kInts);
         Tensor first = grads[0].defined() ? grads[0].to(at::kFloat) : at::zeros({}, stats.options());
         const Tensor out = grad_like(x);
@@ -259,7 +284,7 @@ struct FromStats : Node {
             a = per_row(coef, "coefficients", x, kF32);
         }
         check(mamw_logits_grad(&rows, &at, ignore_index, float(temperature), ptr<float>(stats), &a,
-                               second ? &h : nullptr, ptr<float>(entropy), by_row ? nullptr : ptr<float>(first),
+                               second ? &h : nullptr, ptr<float>(h_out), by_row ? nullptr : ptr<float>(first),
                                ptr(out), stream_of(x)),
               name().c_str());
         return out;
@@ -267,11 +292,11 @@ struct FromStats : Node {
 
     void release_variables() override {
         std::lock_guard<std::mutex> guard(lock);
-        logits.reset_data();
-        tokens.reset_data();
+        logits.reset();
+        tokens.reset();
+        entropy.reset();
         stats = Tensor();
         if (coef.defined()) coef = floats({0}, coef);
-        if (entropy.defined()) entropy = Tensor();
     }
 };
 
@@ -359,10 +384,11 @@ PyObject* token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     if (grad) {
         auto node = node_of<TokenLogprobsBackward>(logits);
-        node->logits = SavedVariable(logits, false);
-        node->tokens = keep(tokens);
+        node->logits = Kept(logits, true);
+        node->tokens = Kept(tokens);
+        node->rows = rows;
         node->stats = stats;
-        node->entropy = entropy.defined() ? entropy.detach() : entropy;
+        if (with_entropy) node->entropy = Kept(entropy.detach());  // an alias: a change in place of the output counts
         node->temperature = temperature;
         node->ignore_index = ignore_index;
         torch::autograd::set_history(logprobs, node);
@@ -384,9 +410,9 @@ Tensor with_node(const Tensor& logits, const std::shared_ptr<N>& node, const mam
         loss = forward(ptr(grad));
     }
     if (node) {
-        node->logits = SavedVariable(logits, false);
+        node->logits = Kept(logits, true);
         for (const Tensor& t : inputs)
-            if (t.defined()) node->inputs.push_back(keep(t));
+            if (t.defined()) node->inputs.emplace_back(t);
         node->rows = rows;
         node->grad = std::move(grad);
         node->workspace = workspace;
@@ -504,8 +530,9 @@ PyObject* preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     if (grad) {
         auto node = node_of<PreferenceLossBackward>(logits);
-        node->logits = SavedVariable(logits, false);
-        node->tokens = keep(tokens);
+        node->logits = Kept(logits, true);
+        node->tokens = Kept(tokens);
+        node->rows = rows;
         node->stats = stats;
         node->coef = coef;
         node->temperature = temperature;
