@@ -202,6 +202,24 @@ def test_policy_many_sequences(gpu, packed):
     check_policy(x, tokens, old, adv, ref, out, x.grad, kl_coef=0.2, sequences=list(zip(bounds, bounds[1:])))
 
 
+def test_sequences_of_one_token(gpu):
+    """Padded sequences of length 1: one value a sequence is one value a row, too."""
+    x, tokens, old, adv, ref = policy_case(6, 130, "bf16", 2, ignored=0.0)
+    x, tokens, old, adv, ref = x[:, None], tokens[:, None], old[:, None], adv[:, None], ref[:, None]
+    tokens[3] = -100
+    x.requires_grad_()
+    out = policy_loss(x, tokens, old, adv, ref_logprobs=ref, kl_coef=0.2, average="sequence")
+    out.loss.backward()
+    check_policy(x, tokens, old, adv, ref, out, x.grad, kl_coef=0.2, sequences=[(i, i + 1) for i in range(6)])
+    y, places = x.detach()[:, 0].requires_grad_(), torch.arange(7, device="cuda")
+    x.grad = None
+    padded = preference_loss(x, tokens, old[:, 0])
+    packed = preference_loss(y, tokens[:, 0], old[:, 0], offsets=places)
+    padded.loss.backward()
+    packed.loss.backward()
+    assert all(torch.equal(p, q) for p, q in zip(padded, packed)) and torch.equal(x.grad[:, 0], y.grad)
+
+
 def test_policy_rows_outside_sequences(gpu):
     """Rows before the first offset and after the last do not count with average="sequence"."""
     x, tokens, old, adv, ref = policy_case(12, 65, "fp32", 5, ignored=0.0)
