@@ -422,7 +422,8 @@ struct HeldRow {
     vec_t v[kVecs];
     Raw<T> single_;
     static constexpr int kGroup = kVecs < 4 ? kVecs : 4, kGroups = kVecs / kGroup;
-    float group_ref[kGroups];  // float: v holds 2^y below its group's, once the statistics are taken
+    // float: v holds 2^y below its group's, once the statistics are taken; -inf of a group of zeros, whatever the row's m
+    float group_ref[kGroups];
 
     __device__ __forceinline__ const void* vecs() const { return row + span.head; }
 
@@ -490,7 +491,8 @@ struct HeldRow {
                     for (int k = 0; k < kVec<T>; ++k) m = fmaxf(m, f[k]);
                 }
                 move_to<false>(st, m, c);
-                const float ref = group_ref[q] = reference(m);
+                group_ref[q] = m;
+                const float ref = reference(m);
 #pragma unroll
                 for (int i = q * kGroup; i < (q + 1) * kGroup; ++i) {
                     asm volatile("" : "+v"(v[i]));
