@@ -7,19 +7,24 @@ at its test."""
 
 import math
 
+import numpy as np
 import pytest
 import torch
 from test_gpu_objectives import (
     DTYPES,
+    U,
     check_distill,
+    check_grad,
     check_policy,
     f64,
+    lp_tol,
     make,
     normal,
+    q_or_one,
 )
 
 from oracle import objectives as ob
-from triton_muon_adamw import distill_loss, policy_loss, token_logprobs
+from triton_muon_adamw import distill_loss, policy_loss, preference_loss, token_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +76,31 @@ def test_distill_of_hidden_entries_at_any_level(gpu, dtype, vocab, level, temper
     loss.backward()
     assert x.grad.isfinite().all() and not x.grad[hidden].any()
     check_distill(x, t, index, lse, None, temperature, loss, x.grad)
+
+
+# ---- logits that are large beside the temperature
+
+@pytest.mark.parametrize("vocab", [33, 1003, 50257])
+@pytest.mark.parametrize("level,temperature", [(1e4, 1.0), (1e5, 1.0), (-1e6, 1.0), (1e7, 1.0), (-1e8, 1.0), (1e6, 0.5),
+                                               (0.0, 2.0**-10), (0.0, 2.0**-14), (0.0, 2.0**-20)])
+def test_logits_large_beside_the_temperature(gpu, vocab, level, temperature):
+    """A logit's difference to the largest one is exact here, so the tolerances are those of any row."""
+    x, tokens, gen = make(8, vocab, "fp32", 85)
+    x = x + level
+    g, h = normal(8, 1.0, gen), normal(8, 0.5, gen)
+    x.requires_grad_()
+    lp, ent = token_logprobs(x, tokens, temperature=temperature, entropy=True)
+    torch.autograd.backward([lp, ent], [g, h])
+    x64, t = f64(x), tokens.cpu().numpy()
+    elp, eent, egrad = ob.token_logprobs(x64, t, temperature, dlogprobs=f64(g), dentropy=f64(h))
+    tol = lp_tol(vocab, elp)
+    assert (np.abs(f64(lp) - elp) <= tol).all()
+    tol_ent = 4 * lp_tol(vocab, eent) * (1 + eent)
+    assert (np.abs(f64(ent) - eent) <= tol_ent).all()
+    a, b = np.abs(f64(g)), np.abs(f64(h))
+    weight = np.sqrt(q_or_one(x64, t, temperature)) / temperature
+    check_grad(x.grad, egrad, (4 * (a + b * (2 + eent)) * lp_tol(vocab, eent) + b * tol_ent)[:, None] * weight)
+    with torch.no_grad():
+        out = preference_loss(x.view(2, 4, -1), tokens.view(2, 4), None, temperature=temperature)
+    sums = elp.reshape(2, 4).sum(-1)
+    assert (np.abs(f64(out.logprobs) - sums) <= tol.reshape(2, 4).sum(-1) + 4 * U * np.abs(sums)).all()

@@ -298,8 +298,8 @@ __device__ __forceinline__ void add(Stats& st, float x, float ref, float c) {
 }
 
 // kCount vectors more.  kQuick: two operations an element less, of eleven, with y = x c - m c in one and without the
-// guard of entropies; not finite, or nothing, where m c overflows or an entry is -inf (see quick_holds).  What the
-// rounding of m c has moved all y by is put right in the sums.
+// guard of entropies; not finite, or nothing, where m c overflows or an entry is -inf, and not exact where m c is large
+// (see quick_holds).  What the rounding of m c has moved all y by is put right in the sums.
 template <typename T, bool kEntropy, bool kQuick, int kCount>
 __device__ __forceinline__ void add_vecs(Stats& st, const vec_t* v, float c) {
     float m = st.m;
@@ -329,18 +329,21 @@ __device__ __forceinline__ void add_vecs(Stats& st, const vec_t* v, float c) {
         }
     }
     if constexpr (kQuick) {
-        const float off = __builtin_fmaf(-ref, c, -shift);  // below 2^-24 |m c|: 2^off is 1 + off ln 2
+        const float off = __builtin_fmaf(-ref, c, -shift);  // below 2^-24 |m c|, and so small that 2^off is 1 + off ln 2
         s = __builtin_fmaf(s * off, kLn2, s);
         st.s += s;
         if (kEntropy) st.sy += __builtin_fmaf(s, off, __builtin_fmaf(sy * off, kLn2, sy));
     }
 }
 
-// Whether quick statistics of a row are the row's: its largest logit has put 1 into s, to within rounding, and
-// nothing overflowed.
+// Whether quick statistics of a row are the row's: its largest logit has put 1 into s, to within rounding, nothing
+// overflowed, and the rounding of m c is at most 2^-13, so that what 1 + off ln 2 leaves out is below 2^-28 of s (at
+// |m c| = 2^17 it would be 2^-18, at 2^24 a sixteenth).  A thread's own m c, below the row's, is either within twice the
+// level as well or so far below that it has no part in s.
+constexpr float kQuickLevel = 4096.f;
 template <bool kEntropy>
-__device__ __forceinline__ bool quick_holds(const Stats& st) {
-    return st.s > 0.5f && st.s < INFINITY && (!kEntropy || fabsf(st.sy) < INFINITY);
+__device__ __forceinline__ bool quick_holds(const Stats& st, float c) {
+    return fabsf(st.m * c) <= kQuickLevel && st.s > 0.5f && st.s < INFINITY && (!kEntropy || fabsf(st.sy) < INFINITY);
 }
 
 // The statistics of vectors from + threadIdx.x, + kThreads_, ... below `to`; change(v, n) is applied to vector n.

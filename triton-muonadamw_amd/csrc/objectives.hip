@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kThreads_) void logprobs_kernel(Rows x, PerRow toke
             return over_block<kEntropy, kThreads_>(over_wave<kEntropy>(st, x.c), x.c, lds[!kQuick]);
         };
         Stats st = stats_of_row(Int<1>());
-        if (!quick_holds<kEntropy>(st)) st = stats_of_row(Int<0>());
+        if (!quick_holds<kEntropy>(st, x.c)) st = stats_of_row(Int<0>());
         const float log_s = logf(st.s);
         lp = (chosen.value() - st.m) * x.inv_t - log_s;
         h = log_s - kLn2 * st.sy / st.s;
