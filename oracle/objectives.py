@@ -131,10 +131,14 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, mask
         if teacher_lse is None:
             g = q * (1.0 if len(t) else 0.0) - target
         else:
-            g = q - target
+            # of sum p (log p - log q): (sum p) q - p; of P (log P - log Q): P (q - the others' own softmax)
+            total = p.sum()
+            g = -target
             if not inside.all():
-                rest_p, rest_q = max(1.0 - p.sum(), SMALLEST_TAIL), q[~inside].sum()
+                rest_p, rest_q = max(1.0 - total, SMALLEST_TAIL), q[~inside].sum()
                 loss += weight * rest_p * np.log(rest_p / rest_q)
                 g[~inside] -= q[~inside] * rest_p / rest_q
+                total += rest_p
+            g += total * q
         grad[r] = weight * g / temperature
     return loss, grad

@@ -104,3 +104,26 @@ def test_logits_large_beside_the_temperature(gpu, vocab, level, temperature):
         out = preference_loss(x.view(2, 4, -1), tokens.view(2, 4), None, temperature=temperature)
     sums = elp.reshape(2, 4).sum(-1)
     assert (np.abs(f64(out.logprobs) - sums) <= tol.reshape(2, 4).sum(-1) + 4 * U * np.abs(sums)).all()
+
+
+# ---- distillation: what the teacher and the student leave to the other entries
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("vocab,k", [(7, 7), (7, 3), (1003, 12), (16390, 12), (50257, 64), (131077, 5)])
+@pytest.mark.parametrize("extra", [0.5, 0.015, -0.4])
+def test_distill_with_probabilities_that_do_not_add_up(gpu, dtype, vocab, k, extra):
+    """A teacher's logits that were rounded after its logsumexp was taken: their probabilities add up to 1 + extra, and
+    the gradient is that of the loss as it is."""
+    x, _, gen = make(5, vocab, dtype, 87)
+    index = torch.rand((5, vocab), device="cuda", generator=gen).argsort(-1)[:, :k].contiguous()
+    t = normal((5, k), 1.5, gen).to(DTYPES[dtype])
+    lse = (torch.logsumexp(t.double() / 2.0, -1) - math.log1p(extra)).float()
+    x.requires_grad_()
+    loss = distill_loss(x, t, index, teacher_lse=lse, temperature=2.0)
+    loss.backward()
+    check_distill(x, t, index, lse, None, 2.0, loss, x.grad)
+    if k == vocab:  # no others: as sharp a tolerance without what they add, (S q_j - p_j) off by 4 d sqrt(q_j) S + 4 ep
+        _, egrad = ob.distill_loss(f64(x), f64(t), index.cpu().numpy(), f64(lse), None, 2.0)
+        size = np.exp(np.stack([ob.log_softmax(row / 2.0) for row in f64(x)]) / 2)
+        ep = U * (k + 8 + 6 * np.abs(f64(t)).max() / 2 + 3 * np.abs(f64(lse)).max())
+        check_grad(x.grad, egrad, 2.0 / 5 * (4 * lp_tol(vocab, 0.0) * (1 + extra) * size + 4 * ep))

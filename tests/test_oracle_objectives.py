@@ -156,3 +156,35 @@ def test_distill_loss(tail):
     assert loss == pytest.approx(value, rel=1e-12)
     np.testing.assert_allclose(grad, expect, rtol=1e-10, atol=1e-13)
     np.testing.assert_allclose(grad, differences(lambda y: ob.distill_loss(y, t, index, **kw)[0], x), atol=1e-8)
+
+
+def with_a_rest(x, t, index, lse):
+    """(the loss by torch, its gradient): sum p (log p - log q) + P (log P - log Q), P at least 2^-20, T = 1."""
+    def fn(xt):
+        lq, total = torch.log_softmax(xt, -1), 0.0
+        for r in range(len(x)):
+            i, logp = torch.tensor(index[r]), torch.tensor(t[r] - lse[r])
+            total = total + (logp.exp() * (logp - lq[r, i])).sum()
+            out = torch.ones(x.shape[1], dtype=torch.bool)
+            out[i] = False
+            if out.any():
+                rest = (1 - logp.exp().sum()).clamp(min=2.0**-20)
+                total = total + rest * (rest.log() - torch.logsumexp(lq[r][out], 0))
+        return total / len(x)
+
+    return auto(fn, x)
+
+
+@pytest.mark.parametrize("k", [4, VOCAB])
+@pytest.mark.parametrize("extra", [0.5, 0.015, -0.4])
+def test_distill_loss_of_probabilities_that_do_not_add_up(k, extra):
+    """To 1 + extra, as a teacher's logits do that were rounded after their logsumexp was taken."""
+    rng, x, _ = inputs(4)
+    index = np.stack([rng.permutation(VOCAB)[:k] for _ in range(ROWS)])
+    t = rng.normal(0, 1, (ROWS, k))
+    lse = np.logaddexp.reduce(t, axis=1) - np.log1p(extra)
+    loss, grad = ob.distill_loss(x, t, index, lse)
+    value, expect = with_a_rest(x, t, index, lse)
+    assert loss == pytest.approx(value, rel=1e-12)
+    np.testing.assert_allclose(grad, expect, rtol=1e-10, atol=1e-13)
+    np.testing.assert_allclose(grad, differences(lambda y: ob.distill_loss(y, t, index, lse)[0], x), atol=1e-8)

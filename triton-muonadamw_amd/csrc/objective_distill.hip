@@ -257,7 +257,9 @@ struct Marks {
 };
 
 // loss = sum p (log p - log q), with kTail + P log(P / Q), where P and Q are what the teacher and the student leave to
-// all other elements; g_j = w (q_j - p_j), and for those others w q_j (1 - P / Q).
+// all other elements; g_j = w (q_j A - p_j), and for those others w q_j (A - P / Q), with A = sum p + P.  That is 1, but for
+// probabilities that add up to more than 1 (logits rounded after their lse was taken; P is at least 2^-20 then), and
+// to less where there are no others.
 //
 // kTail: the teacher's entries are taken out of the row and their sum is added from the gathered logits, so that the
 // sum over all others is not the small difference of two large ones.
@@ -381,14 +383,15 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
     // sum p (log p - log q), with log q = (x - m) / T - log s
     float loss = teacher.plogp - all_parts.px * x.inv_t + teacher.sum_p * logf(s);
     float share = teacher.entries > 0 ? 1.f : 0.f;  // of q_j outside the teacher's entries
-    const float in = kTail ? 1.f : share;
+    float in = share;                               // of q_j at them
     if (teacher.entries == 0) loss = 0.f;
     if constexpr (kTail) {
-        share = 1.f;
+        in = teacher.sum_p;
         if (teacher.entries < x.vocab) {
             const float rest_q = all_parts.s / s, rest_p = fmaxf(1.f - teacher.sum_p, kSmallestTail);
             loss += rest_p * logf(rest_p / rest_q);
-            share = 1.f - rest_p / rest_q;
+            in += rest_p;
+            share = in - rest_p / rest_q;
         }
     }
     if (g) {
