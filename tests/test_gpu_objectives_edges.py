@@ -127,3 +127,22 @@ def test_distill_with_probabilities_that_do_not_add_up(gpu, dtype, vocab, k, ext
         size = np.exp(np.stack([ob.log_softmax(row / 2.0) for row in f64(x)]) / 2)
         ep = U * (k + 8 + 6 * np.abs(f64(t)).max() / 2 + 3 * np.abs(f64(lse)).max())
         check_grad(x.grad, egrad, 2.0 / 5 * (4 * lp_tol(vocab, 0.0) * (1 + extra) * size + 4 * ep))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("vocab", [257, 1003, 4099, 16390, 50257, 131077])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_of_entries_at_the_lowest_value(gpu, dtype, vocab, tail):
+    """Twelve entries a row are visible, six of them the teacher's; all others are at the type's lowest value, so most
+    threads see nothing else."""
+    x, _, gen = make(12, vocab, dtype, 93)
+    seen = torch.rand((12, vocab), device="cuda", generator=gen).argsort(-1)[:, :12].contiguous()
+    hidden = torch.ones((12, vocab), dtype=torch.bool, device="cuda").scatter_(1, seen, False)
+    x = x.masked_fill(hidden, torch.finfo(x.dtype).min).requires_grad_()
+    index = seen[:, :6].contiguous()
+    t = normal((12, 6), 1.5, gen)
+    lse = torch.logsumexp(t, -1) + 0.3 if tail else None
+    loss = distill_loss(x, t, index, teacher_lse=lse)
+    loss.backward()
+    check_distill(x, t, index, lse, None, 1.0, loss, x.grad)
+    assert not x.grad[hidden].any()

@@ -171,25 +171,35 @@ struct Distill {
     const TeacherRow* info;
 };
 
-// A wave's part of a row: its statistics, of the teacher's entries alone the sum s_in of 2^y, the sum p of their
-// probabilities and px of p (x - m).
+// A wave's part of a row: its statistics; of the teacher's entries alone the largest logit `top`, the sum s_in of 2^y,
+// the sum p of their probabilities and px of p (x - top).
 struct Parts {
-    float m, s, s_in, p, px;
+    float m, s, top, s_in, p, px;
 };
 
+// p (from - to): nothing where p is, however far apart the two.
+__device__ __forceinline__ float moved(float p, float from, float to) {
+    return p == 0.f ? 0.f : p * (reference(from) - reference(to));
+}
+
+// p (x - top) goes by the entries' own largest logit: a wave may see nothing but the type's lowest value in the row, and
+// a difference to that would have lost x.
 template <int kThreads_>
 __device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* lds) {
     constexpr int kN = kThreads_ / 64;
     if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = mine;
     __syncthreads();
     mine = lds[threadIdx.x % kN];
-    float m = mine.m;
+    float m = mine.m, top = mine.top;
 #pragma unroll
-    for (int o = kN / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    for (int o = kN / 2; o >= 1; o >>= 1) {
+        m = fmaxf(m, __shfl_xor(m, o, 64));
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+    }
     const float f = __builtin_amdgcn_exp2f(fmaxf(below(mine.m, reference(m), c), -1e30f));
     mine.s *= f;
     mine.s_in *= f;
-    mine.px += mine.p * (reference(mine.m) - reference(m));
+    mine.px += moved(mine.p, mine.top, top);
 #pragma unroll
     for (int o = kN / 2; o >= 1; o >>= 1) {
         mine.s += __shfl_xor(mine.s, o, 64);
@@ -198,6 +208,7 @@ __device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* ld
         mine.px += __shfl_xor(mine.px, o, 64);
     }
     mine.m = m;
+    mine.top = top;
     return mine;
 }
 
@@ -360,28 +371,28 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
             }
     };
     Stats wave = held.stats(x.c, hold, change);
-    if constexpr (kTail) {
-        float x_top = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < kEntries; ++e)
-            if (index[e] >= 0) x_top = fmaxf(x_top, xs[e].value());
-        move_to<false>(wave, fmaxf(wave.m, wave_max(x_top)), x.c);
-    }
-    const float ref = reference(wave.m);
+    for (int e = 0; e < kEntries; ++e)
+        if (index[e] >= 0) top = fmaxf(top, xs[e].value());
+    top = wave_max(top);
+    if constexpr (kTail) move_to<false>(wave, fmaxf(wave.m, top), x.c);
+    const float ref = reference(wave.m), ref_top = reference(top);
     float s_in = 0.f, sum_p = 0.f, px = 0.f;
 #pragma unroll
     for (int e = 0; e < kEntries; ++e) {
         if (index[e] < 0) continue;
         if (kTail) s_in += __builtin_amdgcn_exp2f(below(xs[e].value(), ref, x.c));
         sum_p += probs[e];
-        px += probs[e] > 0.f ? probs[e] * (xs[e].value() - ref) : probs[e];  // 0 * -inf; NaN stays
+        px += probs[e] > 0.f ? probs[e] * (xs[e].value() - ref_top) : probs[e];  // 0 * -inf; NaN stays
     }
     const Parts all_parts = parts_over_block<kThreads_>(
-        {wave.m, wave.s, wave_sum(s_in), wave_sum(sum_p), wave_sum(px)}, x.c, lds);
+        {wave.m, wave.s, top, wave_sum(s_in), wave_sum(sum_p), wave_sum(px)}, x.c, lds);
     const float m = all_parts.m, s = all_parts.s + all_parts.s_in, inv_s = 1.f / s;
     const float count = counted.all();
     // sum p (log p - log q), with log q = (x - m) / T - log s
-    float loss = teacher.plogp - all_parts.px * x.inv_t + teacher.sum_p * logf(s);
+    const float px_m = all_parts.px + moved(all_parts.p, all_parts.top, m);
+    float loss = teacher.plogp - px_m * x.inv_t + teacher.sum_p * logf(s);
     float share = teacher.entries > 0 ? 1.f : 0.f;  // of q_j outside the teacher's entries
     float in = share;                               // of q_j at them
     if (teacher.entries == 0) loss = 0.f;
