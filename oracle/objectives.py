@@ -135,9 +135,9 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, mask
             total = p.sum()
             g = -target
             if not inside.all():
-                rest_p, rest_q = max(1.0 - total, SMALLEST_TAIL), q[~inside].sum()
-                loss += weight * rest_p * np.log(rest_p / rest_q)
-                g[~inside] -= q[~inside] * rest_p / rest_q
+                rest_p, log_rest = max(1.0 - total, SMALLEST_TAIL), np.logaddexp.reduce(logq[~inside])
+                loss += weight * rest_p * (np.log(rest_p) - log_rest)
+                g[~inside] -= rest_p * np.exp(logq[~inside] - log_rest)
                 total += rest_p
             g += total * q
         grad[r] = weight * g / temperature

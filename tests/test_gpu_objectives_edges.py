@@ -130,6 +130,45 @@ def test_distill_with_probabilities_that_do_not_add_up(gpu, dtype, vocab, k, ext
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("vocab", [300, 1003, 16390, 50257, 131077])
+@pytest.mark.parametrize("gap,temperature", [(80.0, 1.0), (110.0, 1.0), (900.0, 1.0), (200.0, 0.125), (5000.0, 4.0)])
+def test_distill_with_a_rest_far_below(gpu, dtype, vocab, gap, temperature):
+    """All other logits lie `gap` T below the teacher's entries: Q underflows, log Q and the others' gradient do not.
+
+    With r the softmax over the others alone, d' the error of log r and of log Q's two logarithms, ep that of a
+    probability of the teacher's: P log(P / Q) is off by P (d' + 3 u |log Q|) + ep (|log P / Q| + 1), the gradient of
+    the others, w (q_j (S + P) - P r_j), by w sqrt(r_j) (4 d' P + ep)."""
+    x, _, gen = make(4, vocab, "fp32", 89)
+    index = torch.rand((4, vocab), device="cuda", generator=gen).argsort(-1)[:, :6].contiguous()
+    x.scatter_(1, index, gap + normal((4, 6), 1.0, gen))
+    x = (x * temperature).to(DTYPES[dtype])
+    t = normal((4, 6), 1.5, gen) * temperature
+    lse = (torch.logsumexp(t.double() / temperature, -1) + 0.2).float()
+    x.requires_grad_()
+    loss = distill_loss(x, t, index, teacher_lse=lse, temperature=temperature)
+    loss.backward()
+    x64, t64, i = f64(x), f64(t) / temperature, index.cpu().numpy()
+    eloss, egrad = ob.distill_loss(x64, f64(t), i, f64(lse), None, temperature)
+    outside = np.ones(x64.shape, bool)
+    np.put_along_axis(outside, i, False, 1)
+    logq = np.stack([ob.log_softmax(row / temperature) for row in x64])
+    log_rest = np.array([np.logaddexp.reduce(l[o]) for l, o in zip(logq, outside)])
+    logr = np.where(outside, logq - log_rest[:, None], -np.inf)
+    p = np.exp(t64 - f64(lse)[:, None])
+    rest_p = 1.0 - p.sum(-1)
+    ep = U * (6 + 8 + 6 * np.abs(t64).max() + 3 * np.abs(f64(lse)).max())
+    d = lp_tol(vocab, np.maximum(np.abs(np.take_along_axis(logq, i, 1)).max(-1), 0.0))
+    dr = 2 * lp_tol(vocab, 0.0)
+    row = (d + ep * (np.abs(np.take_along_axis(logq, i, 1)).max() + np.abs(t64).max() + 1) +
+           rest_p * (dr + 3 * U * np.abs(log_rest)) + ep * (np.abs(np.log(rest_p) - log_rest) + 1))
+    assert abs(loss.item() - eloss) <= 2 * temperature**2 * row.max()
+    w = temperature / 4
+    tol = w * (4 * d[:, None] * np.exp(logq / 2) + np.exp(logr / 2) * (4 * dr * rest_p + ep)[:, None])
+    np.put_along_axis(tol, i, np.take_along_axis(tol, i, 1) + 4 * w * ep, 1)
+    check_grad(x.grad, egrad, tol)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("vocab", [257, 1003, 4099, 16390, 50257, 131077])
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_of_entries_at_the_lowest_value(gpu, dtype, vocab, tail):

@@ -188,3 +188,17 @@ def test_distill_loss_of_probabilities_that_do_not_add_up(k, extra):
     assert loss == pytest.approx(value, rel=1e-12)
     np.testing.assert_allclose(grad, expect, rtol=1e-10, atol=1e-13)
     np.testing.assert_allclose(grad, differences(lambda y: ob.distill_loss(y, t, index, lse)[0], x), atol=1e-8)
+
+
+@pytest.mark.parametrize("gap", [30.0, 2000.0])
+def test_distill_loss_of_a_rest_far_below(gap):
+    """The student leaves next to nothing to the other entries: in 64 bits, too, it may underflow."""
+    rng, x, _ = inputs(5)
+    index = np.stack([rng.permutation(VOCAB)[:4] for _ in range(ROWS)])
+    np.put_along_axis(x, index, np.take_along_axis(x, index, 1) + gap, 1)
+    t = rng.normal(0, 1, (ROWS, 4))
+    lse = np.logaddexp.reduce(t, axis=1) + 0.2
+    loss, grad = ob.distill_loss(x, t, index, lse)
+    value, expect = with_a_rest(x, t, index, lse)
+    assert loss == pytest.approx(value, rel=1e-12)
+    np.testing.assert_allclose(grad, expect, rtol=1e-10, atol=1e-13)

@@ -171,11 +171,16 @@ struct Distill {
     const TeacherRow* info;
 };
 
-// A wave's part of a row: its statistics; of the teacher's entries alone the largest logit `top`, the sum s_in of 2^y,
-// the sum p of their probabilities and px of p (x - top).
+// A wave's part of a row: its statistics (kTail: without the teacher's entries); of those entries alone the largest
+// logit `top` and, below it, the sum s_in of 2^y; the sum p of their probabilities and px of p (x - top).
 struct Parts {
     float m, s, top, s_in, p, px;
 };
+
+// 2^y of `from` below a larger `to`; finite, for sums that are 0.
+__device__ __forceinline__ float factor(float from, float to, float c) {
+    return __builtin_amdgcn_exp2f(below(from, reference(to), c));
+}
 
 // p (from - to): nothing where p is, however far apart the two.
 __device__ __forceinline__ float moved(float p, float from, float to) {
@@ -196,9 +201,8 @@ __device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* ld
         m = fmaxf(m, __shfl_xor(m, o, 64));
         top = fmaxf(top, __shfl_xor(top, o, 64));
     }
-    const float f = __builtin_amdgcn_exp2f(fmaxf(below(mine.m, reference(m), c), -1e30f));
-    mine.s *= f;
-    mine.s_in *= f;
+    mine.s *= factor(mine.m, m, c);
+    mine.s_in *= factor(mine.top, top, c);
     mine.px += moved(mine.p, mine.top, top);
 #pragma unroll
     for (int o = kN / 2; o >= 1; o >>= 1) {
@@ -370,49 +374,51 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
                 if (bits) Mark::leave_out(v, bits);
             }
     };
-    Stats wave = held.stats(x.c, hold, change);
+    const Stats wave = held.stats(x.c, hold, change);
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kEntries; ++e)
         if (index[e] >= 0) top = fmaxf(top, xs[e].value());
     top = wave_max(top);
-    if constexpr (kTail) move_to<false>(wave, fmaxf(wave.m, top), x.c);
-    const float ref = reference(wave.m), ref_top = reference(top);
-    float s_in = 0.f, sum_p = 0.f, px = 0.f;
+    const float ref_top = reference(top);
+    float s_in = 0.f, sum_p = 0.f, px_in = 0.f;
 #pragma unroll
     for (int e = 0; e < kEntries; ++e) {
         if (index[e] < 0) continue;
-        if (kTail) s_in += __builtin_amdgcn_exp2f(below(xs[e].value(), ref, x.c));
+        if (kTail) s_in += __builtin_amdgcn_exp2f(below(xs[e].value(), ref_top, x.c));
         sum_p += probs[e];
-        px += probs[e] > 0.f ? probs[e] * (xs[e].value() - ref_top) : probs[e];  // 0 * -inf; NaN stays
+        px_in += probs[e] > 0.f ? probs[e] * (xs[e].value() - ref_top) : probs[e];  // 0 * -inf; NaN stays
     }
     const Parts all_parts = parts_over_block<kThreads_>(
-        {wave.m, wave.s, top, wave_sum(s_in), wave_sum(sum_p), wave_sum(px)}, x.c, lds);
-    const float m = all_parts.m, s = all_parts.s + all_parts.s_in, inv_s = 1.f / s;
-    const float count = counted.all();
-    // sum p (log p - log q), with log q = (x - m) / T - log s
-    const float px_m = all_parts.px + moved(all_parts.p, all_parts.top, m);
-    float loss = teacher.plogp - px_m * x.inv_t + teacher.sum_p * logf(s);
-    float share = teacher.entries > 0 ? 1.f : 0.f;  // of q_j outside the teacher's entries
-    float in = share;                               // of q_j at them
-    if (teacher.entries == 0) loss = 0.f;
+        {wave.m, wave.s, top, wave_sum(s_in), wave_sum(sum_p), wave_sum(px_in)}, x.c, lds);
+    // m, rest: of what the row holds; all, s: with the teacher's entries
+    const float m = all_parts.m, rest = all_parts.s, all = kTail ? fmaxf(m, all_parts.top) : m;
+    const float m_to_all = kTail ? factor(m, all, x.c) : 1.f;
+    const float s = kTail ? rest * m_to_all + all_parts.s_in * factor(all_parts.top, all, x.c) : rest, inv_s = 1.f / s;
+    // sum p (log p - log q), with log q = (x - all) / T - log s
+    const float px = all_parts.px + moved(all_parts.p, all_parts.top, all);
+    float loss = teacher.entries > 0 ? teacher.plogp - px * x.inv_t + teacher.sum_p * logf(s) : 0.f;
+    float in = teacher.entries > 0 ? 1.f : 0.f;  // times inv_s 2^y: A q_j
+    float outside = in * inv_s;                     // times 2^y below m: A q_j - P q_j / Q, outside the entries
     if constexpr (kTail) {
         in = teacher.sum_p;
         if (teacher.entries < x.vocab) {
-            const float rest_q = all_parts.s / s, rest_p = fmaxf(1.f - teacher.sum_p, kSmallestTail);
-            loss += rest_p * logf(rest_p / rest_q);
+            // Q = rest 2^(m below all) / s may be beyond what 32 bits hold, its logarithm and q_j / Q = 2^y / rest are not
+            const float rest_p = fmaxf(1.f - teacher.sum_p, kSmallestTail);
+            loss += rest_p * (logf(rest_p * s / rest) + (all - m) * x.inv_t);
             in += rest_p;
-            share = in - rest_p / rest_q;
+            outside = in * m_to_all * inv_s - rest_p / rest;
         }
     }
+    const float count = counted.all();
     if (g) {
         const float w = teacher.beyond ? NAN : f * p.scale * p.temperature / count;
-        held.write(g, w * share * inv_s, m, x.c, change);
+        held.write(g, w * outside, m, x.c, change);
         __syncthreads();  // then the entries themselves, over what was written there
 #pragma unroll
         for (int e = 0; e < kEntries; ++e)
             if (index[e] >= 0)
-                g[index[e]] = narrow<T>(w * (in * inv_s * __builtin_amdgcn_exp2f(below(xs[e].value(), m, x.c)) - probs[e]));
+                g[index[e]] = narrow<T>(w * (in * inv_s * __builtin_amdgcn_exp2f(below(xs[e].value(), all, x.c)) - probs[e]));
     }
     put_part(out, r, (teacher.beyond ? NAN : loss) / count, 0.f, 0.f);
 }
