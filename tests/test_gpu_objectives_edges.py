@@ -168,6 +168,26 @@ def test_distill_with_a_rest_far_below(gpu, dtype, vocab, gap, temperature):
     check_grad(x.grad, egrad, tol)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+def test_padding_may_point_anywhere(gpu, tail):
+    """An entry with a logit of -inf is left out whatever its index."""
+    x, _, gen = make(4, 1003, "fp32", 91)
+    index = torch.rand((4, 1003), device="cuda", generator=gen).argsort(-1)[:, :9].contiguous()
+    t = normal((4, 9), 1.5, gen)
+    t[:, 6:] = -math.inf
+    lse = torch.logsumexp(t, -1) + 0.3 if tail else None
+    losses, grads = [], []
+    for padding in (-1, 0, 1003, 1 << 40):
+        index[:, 6:] = padding
+        y = x.clone().requires_grad_()
+        loss = distill_loss(y, t, index, teacher_lse=lse)
+        loss.backward()
+        check_distill(y, t, index.clamp(max=1002), lse, None, 1.0, loss, y.grad)
+        losses.append(loss.detach())
+        grads.append(y.grad)
+    assert all(torch.equal(p, losses[0]) for p in losses) and all(torch.equal(g, grads[0]) for g in grads)
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("vocab", [257, 1003, 4099, 16390, 50257, 131077])
 @pytest.mark.parametrize("tail", [False, True])

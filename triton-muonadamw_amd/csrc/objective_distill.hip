@@ -73,8 +73,8 @@ __global__ __launch_bounds__(64 * kTeacherRows) void teacher_kernel(Rows x, Teac
                 const bool is = k < a.k;
                 t[e] = is ? load_float(a.logits, tl + k) : -INFINITY;
                 const int64_t j = is ? load_int(a.indices, ti + k) : -1;
-                beyond |= j >= x.vocab;
-                const bool in = j >= 0 && j < x.vocab && t[e] != -INFINITY;
+                const bool given = j >= 0 && t[e] != -INFINITY, in = given && j < x.vocab;
+                beyond |= given && !in;
                 idx[e] = in ? int32_t(j) : kPadding;
                 if (in) top = fmaxf(top, t[e]);
             }
