@@ -205,3 +205,18 @@ def test_distill_of_entries_at_the_lowest_value(gpu, dtype, vocab, tail):
     loss.backward()
     check_distill(x, t, index, lse, None, 1.0, loss, x.grad)
     assert not x.grad[hidden].any()
+
+
+# ---- preference
+
+@pytest.mark.parametrize("smoothing", [0.0, 1.0])
+def test_an_impossible_sequence_is_no_contradiction(gpu, smoothing):
+    """A token of no probability in the sequence that ought to be unlikely: its reward is -inf, the loss 0."""
+    x, tokens, _ = make(4, 77, "fp32", 95, ignored=0.0)
+    unlikely = 2 if smoothing == 0.0 else 0
+    x[unlikely, tokens[unlikely]] = -math.inf
+    x = x.view(2, 2, -1).requires_grad_()
+    out = preference_loss(x, tokens.view(2, 2), None, label_smoothing=smoothing)
+    grad, = torch.autograd.grad(out.loss, x)
+    assert out.loss == 0 and out.rewards[unlikely // 2] == -math.inf
+    assert not grad.any()

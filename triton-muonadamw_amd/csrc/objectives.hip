@@ -300,7 +300,9 @@ __global__ __launch_bounds__(kThreads) void pairs_kernel(Rows x, Preference p, c
     float loss, slope;  // d loss / d h
     if (p.kind == MAMW_SIGMOID) {
         const float soft = log1pf(expf(-fabsf(h)));  // -log sigmoid(|h|)
-        loss = (1.f - p.smoothing) * (soft + fmaxf(-h, 0.f)) + p.smoothing * (soft + fmaxf(h, 0.f));
+        // h may be infinite (a token of no probability): what has no weight adds nothing
+        loss = p.smoothing < 1.f ? (1.f - p.smoothing) * (soft + fmaxf(-h, 0.f)) : 0.f;
+        if (p.smoothing > 0.f) loss += p.smoothing * (soft + fmaxf(h, 0.f));
         slope = p.smoothing - 1.f / (1.f + expf(h));
     } else if (p.kind == MAMW_IPO) {
         const float d = (h - 0.5f) / p.beta;
