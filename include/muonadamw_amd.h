@@ -354,7 +354,8 @@ int mamw_token_logprobs(const mamw_rows* logits, const mamw_per_row* tokens,
 
 /* grad_j = (a [j = token] - q_j (a + h (log q_j + entropy))) / T with
  * a = scale * coef[r], h = scale * entropy_coef[r] (no such term where
- * entropy_coef is NULL) and *scale on the device (NULL: 1).                   */
+ * entropy_coef is NULL) and *scale on the device (NULL: 1).  A row whose a and h
+ * are 0 is not read and gets zeros, whatever it holds.                        */
 int mamw_logits_grad(const mamw_rows* logits, const mamw_per_row* tokens,
                      int64_t ignore_index, float temperature,
                      const float* stats, const mamw_per_row* coef,
@@ -393,7 +394,8 @@ int mamw_policy_grad(const mamw_rows* logits, const mamw_policy* p, const float*
 
 /* Preference loss over pairs of sequences, i < pairs = sequences / 2 against
  * i + pairs.  With L_s the sum of log q_token over the rows of sequence s that count
- * (their mean with length_average; 0 where there are none),
+ * (their mean with length_average; 0 where there are none; rows in no sequence
+ * do not count),
  *     rewards_s = beta (L_s - ref_s),  h = rewards_i - rewards_{i+pairs},
  *     MAMW_SIGMOID: -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h)
  *     MAMW_IPO:     (h / beta - 1 / (2 beta))^2

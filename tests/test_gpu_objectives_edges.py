@@ -220,3 +220,23 @@ def test_an_impossible_sequence_is_no_contradiction(gpu, smoothing):
     grad, = torch.autograd.grad(out.loss, x)
     assert out.loss == 0 and out.rewards[unlikely // 2] == -math.inf
     assert not grad.any()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_rows_outside_the_pairs_do_not_count(gpu, dtype, bad):
+    """Rows before the first offset and after the last, whatever they hold."""
+    x, tokens, _ = make(12, 1003, dtype, 97, ignored=0.0)
+    offsets = torch.tensor([2, 5, 9], device="cuda")
+    y = x[2:9].clone().requires_grad_()
+    expect = preference_loss(y, tokens[2:9].clone(), None, offsets=offsets - 2)
+    expect.loss.backward()
+    x[:2] = x[9:] = bad
+    x.requires_grad_()
+    out = preference_loss(x, tokens, None, offsets=offsets)
+    out.loss.backward()
+    d = 16 * lp_tol(1003, 40.0)
+    for p, q in zip(out, expect):  # to within the place of the rows in memory
+        assert (np.abs(f64(p) - f64(q)) <= d * np.maximum(1.0, np.abs(f64(q)))).all()
+    assert not x.grad[:2].any() and not x.grad[9:].any()
+    check_grad(x.grad[2:9], f64(y.grad), d + 2.0**-8 * np.abs(f64(y.grad)))

@@ -46,7 +46,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
                    entropy: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Log-probability of ``tokens`` under ``softmax(logits / temperature)``,
     float32, 0 where the token is ``ignore_index``; with ``entropy`` also the
-    distribution's entropy.  Both are differentiable."""
+    distribution's entropy.  Both are differentiable; rows whose gradients from
+    outside are 0 get one of 0, whatever their logits."""
     out = _lib.objectives().token_logprobs(logits, tokens, temperature, ignore_index, entropy)
     return out if entropy else out[0]
 
@@ -85,8 +86,8 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logprobs: to
     ``kind``: ``"sigmoid"`` ``-log sigmoid(h)`` (with ``label_smoothing`` e,
     ``1 - e`` of it and ``e`` of ``-log sigmoid(-h)``), ``"ipo"``
     ``(h / beta - 1 / (2 beta))**2``, ``"hinge"`` ``max(0, 1 - h)``; the loss is
-    the mean over the pairs.  Sequences as in :func:`policy_loss`;
-    ``ref_logprobs`` holds one value for each, ``None`` for 0."""
+    the mean over the pairs.  Sequences as in :func:`policy_loss`; rows in none of
+    them do not count.  ``ref_logprobs`` holds one value for each, ``None`` for 0."""
     if kind not in _KINDS:
         raise ValueError(f"kind must be one of {sorted(_KINDS)} (got {kind!r})")
     return PreferenceLoss(*_lib.objectives().preference_loss(
