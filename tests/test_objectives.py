@@ -269,3 +269,24 @@ def test_a_missing_native_module_is_an_error(monkeypatch):
     monkeypatch.setitem(sys.modules, "triton_muon_adamw._objectives", None)
     with pytest.raises(RuntimeError, match="_objectives cannot be used"):
         logprobs()
+
+
+def test_abi_types_that_are_none():
+    """In a process of its own: what ends it is not an error status."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = f"""
+import sys
+sys.path[:0] = {[str(Path(__file__).parent), *sys.path]!r}
+from test_objectives import *
+for kind, make, name in [("policy", a_policy, "old_logprobs"), ("policy", a_policy, "advantages"),
+                         ("policy", a_policy, "ref_logprobs"), ("distill", a_distill, "teacher_lse"),
+                         ("distill", a_distill, "mask")]:
+    for number in (-1, 6, 1 << 30):
+        assert ws_bytes(kind, rows(), make(**{{name: per_row(number)}}))[0] == HYPER, (name, number)
+print("refused")
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert (res.returncode, res.stdout.strip()) == (0, "refused"), res.stderr[-500:]

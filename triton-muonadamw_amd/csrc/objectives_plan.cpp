@@ -62,9 +62,10 @@ int check_rows(const mamw_rows* x, const void* grad) {
 
 int check_per_row(const mamw_per_row& a, bool needed, int32_t type, int32_t other_type) {
     if (!a.data) return needed ? MAMW_ERR_NULL : MAMW_OK;
-    if (a.reserved || (a.type != type && a.type != other_type)) return MAMW_ERR_HYPER;
+    const size_t size = element_size(a.type);  // 0: no type, whatever the caller's is compared with
+    if (a.reserved || size == 0 || (a.type != type && a.type != other_type)) return MAMW_ERR_HYPER;
     if (a.outer_stride < 0 || a.inner_stride < 0) return MAMW_ERR_SHAPE;
-    if (!aligned(a.data, element_size(a.type))) return MAMW_ERR_ALIGN;
+    if (!aligned(a.data, size)) return MAMW_ERR_ALIGN;
     return MAMW_OK;
 }
 
