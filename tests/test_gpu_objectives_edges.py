@@ -20,6 +20,7 @@ from test_gpu_objectives import (
     lp_tol,
     make,
     normal,
+    policy_case,
     q_or_one,
 )
 
@@ -240,3 +241,92 @@ def test_rows_outside_the_pairs_do_not_count(gpu, dtype, bad):
         assert (np.abs(f64(p) - f64(q)) <= d * np.maximum(1.0, np.abs(f64(q)))).all()
     assert not x.grad[:2].any() and not x.grad[9:].any()
     check_grad(x.grad[2:9], f64(y.grad), d + 2.0**-8 * np.abs(f64(y.grad)))
+
+
+# ---- what backward keeps
+
+ROWS, WIDTH, VOCAB = 24, 16, 5003
+
+
+def losses():
+    _, tokens, old, adv, ref = policy_case(ROWS, VOCAB, "bf16", 99)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    index = torch.rand((ROWS, VOCAB), device="cuda", generator=gen).argsort(-1)[:, :9].contiguous()
+    t = normal((ROWS, 9), 1.0, gen)
+    lse = torch.logsumexp(t, -1) + 0.3
+    places = torch.tensor([0, 5, 11, 12, ROWS], dtype=torch.int32, device="cuda")
+    return {
+        "logprobs": lambda x: (lambda o: o[0].sum() + 0.1 * o[1].sum())(token_logprobs(x, tokens, entropy=True)),
+        "policy": lambda x: policy_loss(x, tokens, old, adv, ref_logprobs=ref, kl_coef=0.1, average="sequence",
+                                        offsets=places).loss,
+        "policy rows": lambda x: policy_loss(x.view(4, 6, VOCAB), tokens.view(4, 6), old.view(4, 6), adv[:4, None]).loss,
+        "preference": lambda x: preference_loss(x, tokens, None, offsets=places).loss,
+        "distill": lambda x: distill_loss(x, t, index, mask=tokens != -100),
+        "rest": lambda x: distill_loss(x, t, index, teacher_lse=lse),
+    }
+
+
+@pytest.mark.parametrize("which", ["logprobs", "policy", "policy rows", "preference", "distill", "rest"])
+@pytest.mark.parametrize("factor", [1.0, 3.0])
+@pytest.mark.parametrize("how", ["checkpoint", "cpu"])
+def test_saved_tensors_kept_elsewhere(gpu, which, factor, how):
+    """Recomputed by a checkpoint or brought back from host memory, the logits lie elsewhere in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+
+    loss_of = losses()[which]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    hidden = normal((ROWS, WIDTH), 1.0, gen)
+    head = normal((WIDTH, VOCAB), 0.5, gen).bfloat16().requires_grad_()
+
+    def step(h):
+        return loss_of(h.bfloat16() @ head)
+
+    def grads(run):
+        h = hidden.clone().requires_grad_()
+        loss = run(h)
+        junk = [torch.full((1 << 18,), math.nan, device="cuda") for _ in range(8)]  # where freed logits were
+        return [loss.detach(), *torch.autograd.grad(loss * factor, [h, head])], junk
+
+    def on_cpu(h):
+        with torch.autograd.graph.save_on_cpu():
+            return step(h)
+
+    expect, _ = grads(step)
+    got, _ = grads((lambda h: checkpoint(step, h, use_reentrant=False)) if how == "checkpoint" else on_cpu)
+    for p, q in zip(got, expect):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("which", ["logprobs", "policy", "preference", "distill"])
+def test_saved_strided_tensors_come_back_dense(gpu, which):
+    loss_of = losses()[which]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    wide = normal((ROWS, VOCAB + 13), 2.0, gen).bfloat16()
+    grads = []
+    for hooked in (False, True):
+        x = wide.clone().requires_grad_()
+        if hooked:
+            with torch.autograd.graph.save_on_cpu():
+                loss = loss_of(x[:, 3:VOCAB + 3])
+        else:
+            loss = loss_of(x[:, 3:VOCAB + 3])
+        grads.append(torch.autograd.grad(3 * loss, x)[0])
+    d = 16 * lp_tol(VOCAB, 40.0)
+    assert f64(grads[0]).any()
+    check_grad(grads[1], f64(grads[0]), d * np.sqrt(np.abs(f64(grads[0]))) + 2.0**-8 * np.abs(f64(grads[0])))
+
+
+@pytest.mark.parametrize("which", ["logprobs", "policy", "preference", "distill"])
+def test_saved_tensors_kept_elsewhere_are_let_go(gpu, which):
+    """Neither the logits nor a gradient of their size stays on the device."""
+    loss_of = losses()[which]
+    x = normal((ROWS, VOCAB), 2.0, torch.Generator(device="cuda").manual_seed(5)).requires_grad_()
+    loss_of(x * 1.0)  # what is allocated once
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        loss = loss_of(x * 1.0)
+    assert torch.cuda.memory_allocated() - before < x.numel() * 4 // 2
+    first, = torch.autograd.grad(loss, x, retain_graph=True)
+    second, = torch.autograd.grad(loss, x)
+    assert torch.equal(first, second)

@@ -19,6 +19,7 @@
 #include <pybind11/pybind11.h>
 
 #include <mutex>
+#include <tuple>
 
 #include "muonadamw_amd.h"
 
@@ -149,27 +150,39 @@ Tensor bytes(size_t n, const Tensor& like) {
     return at::empty({int64_t(n < 256 ? 256 : n)}, like.options().dtype(at::kByte));
 }
 
-// A tensor that backward reads by the address it had in the forward pass.  Its memory stays, and who has put other
-// memory under it meanwhile (t.data = ..., which no version counter sees) gets an error.
+// A tensor that backward reads.  Where saved-tensor hooks are in force (a checkpoint that computes it again, offloading to
+// host memory) they have it, nothing of it stays here, and it comes back at another address.  Otherwise its memory stays,
+// and who has put other memory under it meanwhile (t.data = ..., which no version counter sees) gets an error.
 struct Kept {
     SavedVariable saved;
     c10::Storage storage;
     const void* data = nullptr;
+    bool hooked = false;
 
-    Kept() = default;
+    Kept() = default;  // of an undefined tensor
     // Of `logits` a gradient is wanted; what is kept of other inputs is their value.
     Kept(const Tensor& t, bool logits = false)
-        : saved(!logits && t.requires_grad() ? t.detach() : t, false), storage(t.storage()), data(t.const_data_ptr()) {}
+        : saved(!logits && t.requires_grad() ? t.detach() : t, false), hooked(saved.has_hooks()) {
+        if (hooked) return;
+        storage = t.storage();
+        data = t.const_data_ptr();
+    }
 
     Tensor unpack() const {
         Tensor t = saved.unpack();  // raises where it was released, or changed in place since
-        TORCH_CHECK(t.const_data_ptr() == data,
+        TORCH_CHECK(hooked || !t.defined() || t.const_data_ptr() == data,
                     "a tensor that the gradient needs was given other memory after the forward pass");
         return t;
     }
-    Tensor unpack(const mamw_rows& rows) const {
+    // Of logits: `rows` are those of the forward pass, and then of the memory that they are in now.
+    Tensor unpack(mamw_rows& rows, const Tensor& like) const {
         Tensor x = unpack();
-        TORCH_CHECK(x.dim() >= 1 && x.size(-1) == rows.vocab && x.numel() == rows.outer * rows.inner * rows.vocab,
+        TORCH_CHECK(x.device() == like.device() && float_type(x.scalar_type()) == rows.type, "logits of the forward pass on ",
+                    like.device(), " came back as ", x.scalar_type(), " on ", x.device());
+        const mamw_rows was = rows;
+        if (x.dim() == 2 || x.dim() == 3) rows = rows_of(x);
+        TORCH_CHECK((x.dim() == 2 || x.dim() == 3) && rows.outer == was.outer && rows.inner == was.inner &&
+                        rows.vocab == was.vocab,
                     "logits changed their shape after the forward pass (now ", x.sizes(), ")");
         return x;
     }
@@ -193,14 +206,16 @@ Tensor once(const Tensor& grad) {
 // A loss whose forward kernel writes the gradient as well, because a row's gradient needs nothing beyond that row.
 // backward hands it out; a gradient of the loss other than 1 has it computed again from the logits with that factor
 // (the device decides, so nothing waits), which rounds once and keeps float16 gradients of a scaled loss from
-// vanishing first.
+// vanishing first.  Where hooks keep the logits, a gradient of their size is not kept beside them: backward computes it.
 struct OnePass : Node {
     std::mutex lock;
     Kept logits;
-    std::vector<Kept> inputs;  // what the description points to
+    std::vector<Kept> inputs;  // what the description points to, in the order of describe()
     mamw_rows rows;
     Tensor grad, workspace;
 
+    // Has the description point to `inputs`, which go with logits x.
+    virtual void describe(const Tensor& x, at::ArrayRef<Tensor> inputs) = 0;
     virtual int again(const float* scale, int unless_one, void* out, mamw_stream_t stream) = 0;
 
     variable_list apply(variable_list&& grads) override {
@@ -211,12 +226,14 @@ struct OnePass : Node {
 
     Tensor gradient(const Tensor& grad_output) {
         at::NoGradGuard no_grad;
-        const Tensor x = logits.unpack(rows);
-        for (auto& i : inputs) i.unpack();
+        const Tensor x = logits.unpack(rows, workspace);
+        c10::SmallVector<Tensor, 5> with;
+        for (auto& i : inputs) with.push_back(i.unpack());
+        describe(x, with);
         const c10::DeviceGuard device(x.device());
         Tensor out = std::move(grad);
         grad = Tensor();
-        const bool fresh = !out.defined();  // the graph was retained and the first one is someone else's now
+        const bool fresh = !out.defined();  // the graph was retained and the first one is someone else's now, or hooks
         if (fresh) out = grad_like(x);
         const Tensor scale = grad_output.to(at::kFloat);
         check(again(ptr<float>(scale), !fresh, ptr(out), stream_of(x)), name().c_str());
@@ -231,9 +248,27 @@ struct OnePass : Node {
     }
 };
 
+// tokens, old_logprobs, advantages, ref_logprobs, offsets (int64)
+void describe_policy(mamw_policy& p, const Tensor& logits, at::ArrayRef<Tensor> inputs) {
+    p.tokens = per_row(inputs[0], "tokens", logits, kInts);
+    p.old_logprobs = per_row(inputs[1], "old_logprobs", logits, kF32);
+    p.advantages = per_row(inputs[2], "advantages", logits, kF32);
+    p.ref_logprobs = per_row(inputs[3], "ref_logprobs", logits, kF32);
+    p.offsets = inputs[4].defined() ? inputs[4].const_data_ptr<int64_t>() : nullptr;
+}
+
+// teacher_logits, teacher_indices, teacher_lse, mask
+void describe_distill(mamw_distill& p, const Tensor& logits, at::ArrayRef<Tensor> inputs) {
+    p.teacher_logits = per_row(inputs[0], "teacher_logits", logits, kFloats, p.k);
+    p.teacher_indices = per_row(inputs[1], "teacher_indices", logits, kInts, p.k);
+    p.teacher_lse = per_row(inputs[2], "teacher_lse", logits, kF32);
+    p.mask = per_row(inputs[3], "mask", logits, kBool);
+}
+
 struct PolicyLossBackward : OnePass {
     mamw_policy desc;
     std::string name() const override { return "PolicyLossBackward"; }
+    void describe(const Tensor& x, at::ArrayRef<Tensor> inputs) override { describe_policy(desc, x, inputs); }
     int again(const float* scale, int unless_one, void* out, mamw_stream_t stream) override {
         return mamw_policy_grad(&rows, &desc, scale, unless_one, out, ptr(workspace), workspace.numel(), stream);
     }
@@ -242,6 +277,7 @@ struct PolicyLossBackward : OnePass {
 struct DistillLossBackward : OnePass {
     mamw_distill desc;
     std::string name() const override { return "DistillLossBackward"; }
+    void describe(const Tensor& x, at::ArrayRef<Tensor> inputs) override { describe_distill(desc, x, inputs); }
     int again(const float* scale, int unless_one, void* out, mamw_stream_t stream) override {
         return mamw_distill_grad(&rows, &desc, scale, unless_one, out, ptr(workspace), workspace.numel(), stream);
     }
@@ -267,7 +303,7 @@ struct FromStats : Node {
 
     Tensor gradient(const variable_list& grads, bool by_row, bool second) {
         at::NoGradGuard no_grad;
-        const Tensor x = logits.unpack(rows), toks = tokens.unpack(), h_out = second ? entropy.unpack() : Tensor();
+        const Tensor x = logits.unpack(rows, stats), toks = tokens.unpack(), h_out = second ? entropy.unpack() : Tensor();
         const c10::DeviceGuard device(x.device());
         const mamw_per_row at = per_row(toks, "tokens", x, kInts);
         Tensor first = grads[0].defined() ? grads[0].to(at::kFloat) : at::zeros({}, stats.options());
@@ -401,18 +437,17 @@ PyObject* token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
 // The forward pass of a loss in one, for `node` (NULL: no gradient).
 template <typename N, typename Fn>
 Tensor with_node(const Tensor& logits, const std::shared_ptr<N>& node, const mamw_rows& rows, const Tensor& workspace,
-                 std::initializer_list<Tensor> inputs, Fn forward) {
+                 at::ArrayRef<Tensor> inputs, Fn forward) {
+    if (node) node->logits = Kept(logits, true);
     Tensor loss, grad;
     {
         pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
-        if (node) grad = grad_like(logits);
+        if (node && !node->logits.hooked) grad = grad_like(logits);
         loss = forward(ptr(grad));
     }
     if (node) {
-        node->logits = Kept(logits, true);
-        for (const Tensor& t : inputs)
-            if (t.defined()) node->inputs.emplace_back(t);
+        for (const Tensor& t : inputs) node->inputs.push_back(t.defined() ? Kept(t) : Kept());
         node->rows = rows;
         node->grad = std::move(grad);
         node->workspace = workspace;
@@ -427,18 +462,14 @@ PyObject* policy_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const Args a{v, n};
     a.expect(13);
-    const Tensor logits = a.tensor(0, "logits"), tokens = a.tensor(1, "tokens"), old = a.tensor(2, "old_logprobs"),
-                 advantages = a.tensor(3, "advantages"), ref = a.maybe_tensor(4, "ref_logprobs");
+    const Tensor logits = a.tensor(0, "logits");
+    Tensor inputs[5] = {a.tensor(1, "tokens"), a.tensor(2, "old_logprobs"), a.tensor(3, "advantages"),
+                        a.maybe_tensor(4, "ref_logprobs"), Tensor()};
     const mamw_rows rows = rows_of(logits);
     mamw_policy p = {};
     p.by_sequence = a.truth(8);
-    const auto [offsets, count] = sequences(a.maybe_tensor(9, "offsets"), logits, p.by_sequence);
-    p.tokens = per_row(tokens, "tokens", logits, kInts);
-    p.old_logprobs = per_row(old, "old_logprobs", logits, kF32);
-    p.advantages = per_row(advantages, "advantages", logits, kF32);
-    p.ref_logprobs = per_row(ref, "ref_logprobs", logits, kF32);
-    p.offsets = offsets.defined() ? offsets.const_data_ptr<int64_t>() : nullptr;
-    p.sequences = count;
+    std::tie(inputs[4], p.sequences) = sequences(a.maybe_tensor(9, "offsets"), logits, p.by_sequence);
+    describe_policy(p, logits, inputs);
     p.kl_coef = float(a.real(5));
     p.clip_low = float(a.real(6));
     p.clip_high = float(a.real(7));
@@ -461,7 +492,7 @@ PyObject* policy_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
         workspace = bytes(need, logits);
         logprobs = floats(logits.sizes().slice(0, logits.dim() - 1), logits);
     }
-    const Tensor loss = with_node(logits, node, rows, workspace, {tokens, old, advantages, ref, offsets}, [&](void* grad) {
+    const Tensor loss = with_node(logits, node, rows, workspace, inputs, [&](void* grad) {
         const Tensor result = floats({3}, logits);
         check(mamw_policy_loss(&rows, &p, ptr<float>(result), ptr<float>(logprobs), grad, ptr(workspace), workspace.numel(),
                                stream_of(logits)),
@@ -548,8 +579,10 @@ PyObject* distill_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const Args a{v, n};
     a.expect(7);
-    const Tensor logits = a.tensor(0, "logits"), lse = a.maybe_tensor(3, "teacher_lse"), mask = a.maybe_tensor(4, "mask");
-    Tensor teacher = a.tensor(1, "teacher_logits").detach(), index = a.tensor(2, "teacher_indices");
+    const Tensor logits = a.tensor(0, "logits");
+    Tensor inputs[4] = {a.tensor(1, "teacher_logits").detach(), a.tensor(2, "teacher_indices"),
+                        a.maybe_tensor(3, "teacher_lse"), a.maybe_tensor(4, "mask")};
+    Tensor &teacher = inputs[0], &index = inputs[1];
     const mamw_rows rows = rows_of(logits);
     const int64_t k = teacher.dim() ? teacher.size(-1) : 0;
     TORCH_CHECK_VALUE(k >= 1 && k <= MAMW_MAX_TEACHER, "teacher_logits must have between 1 and ", MAMW_MAX_TEACHER,
@@ -557,11 +590,8 @@ PyObject* distill_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (k > 1 && teacher.stride(-1) != 1) teacher = teacher.contiguous();
     if (k > 1 && index.dim() && index.stride(-1) != 1) index = index.contiguous();
     mamw_distill p = {};
-    p.teacher_logits = per_row(teacher, "teacher_logits", logits, kFloats, k);
-    p.teacher_indices = per_row(index, "teacher_indices", logits, kInts, k);
-    p.teacher_lse = per_row(lse, "teacher_lse", logits, kF32);
-    p.mask = per_row(mask, "mask", logits, kBool);
     p.k = k;
+    describe_distill(p, logits, inputs);
     p.temperature = float(a.real(5));
     p.scale = float(a.real(6));
     size_t need = 0;
@@ -579,7 +609,7 @@ PyObject* distill_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
         at::AutoDispatchBelowADInplaceOrView below;
         workspace = bytes(need, logits);
     }
-    const Tensor loss = with_node(logits, node, rows, workspace, {teacher, index, lse, mask}, [&](void* grad) {
+    const Tensor loss = with_node(logits, node, rows, workspace, inputs, [&](void* grad) {
         const Tensor result = floats({3}, logits);
         check(mamw_distill_loss(&rows, &p, ptr<float>(result), grad, ptr(workspace), workspace.numel(),
                                 stream_of(logits)),
