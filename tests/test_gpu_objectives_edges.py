@@ -330,3 +330,24 @@ def test_saved_tensors_kept_elsewhere_are_let_go(gpu, which):
     first, = torch.autograd.grad(loss, x, retain_graph=True)
     second, = torch.autograd.grad(loss, x)
     assert torch.equal(first, second)
+
+
+def test_inputs_of_inference_mode(gpu):
+    """What an inference-mode pass computed goes with a loss that is trained on, as a constant."""
+    x, tokens, old, adv, ref = policy_case(8, 1003, "bf16", 101)
+    with torch.inference_mode():
+        kept = [v.clone() for v in (tokens, old, adv, ref)]
+        mask = kept[0] != -100
+        index, top = torch.arange(8, device="cuda")[:, None].clone(), kept[1][:, None].clone()
+    index_, top_ = torch.arange(8, device="cuda")[:, None], old[:, None]
+
+    def run(tokens, old, adv, ref, mask, index, top):
+        y = x.clone().requires_grad_()
+        out = [policy_loss(y, tokens, old, adv, ref_logprobs=ref, kl_coef=0.1).loss, token_logprobs(y, tokens).sum(),
+               distill_loss(y, top, index, mask=mask),
+               preference_loss(y.view(2, 4, -1), tokens.view(2, 4), ref[:2]).loss]
+        return [torch.autograd.grad(3 * v, y)[0] for v in out]
+
+    expect = run(tokens, old, adv, ref, tokens != -100, index_, top_)
+    for p, q in zip(run(*kept, mask, index, top), expect):
+        assert torch.equal(p, q)

@@ -155,20 +155,27 @@ Tensor bytes(size_t n, const Tensor& like) {
 // and who has put other memory under it meanwhile (t.data = ..., which no version counter sees) gets an error.
 struct Kept {
     SavedVariable saved;
+    Tensor constant;  // of inference mode: without a version, it cannot be saved, nor a change of it be noticed
     c10::Storage storage;
     const void* data = nullptr;
     bool hooked = false;
 
     Kept() = default;  // of an undefined tensor
     // Of `logits` a gradient is wanted; what is kept of other inputs is their value.
-    Kept(const Tensor& t, bool logits = false)
-        : saved(!logits && t.requires_grad() ? t.detach() : t, false), hooked(saved.has_hooks()) {
+    Kept(const Tensor& t, bool logits = false) {
+        if (t.is_inference()) {
+            constant = t;
+            return;
+        }
+        saved = SavedVariable(!logits && t.requires_grad() ? t.detach() : t, false);
+        hooked = saved.has_hooks();
         if (hooked) return;
         storage = t.storage();
         data = t.const_data_ptr();
     }
 
     Tensor unpack() const {
+        if (constant.defined()) return constant;
         Tensor t = saved.unpack();  // raises where it was released, or changed in place since
         TORCH_CHECK(hooked || !t.defined() || t.const_data_ptr() == data,
                     "a tensor that the gradient needs was given other memory after the forward pass");
@@ -188,6 +195,7 @@ struct Kept {
     }
     void reset() {
         saved.reset_data();
+        constant = Tensor();
         storage = c10::Storage();
     }
 };
