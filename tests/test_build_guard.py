@@ -154,3 +154,12 @@ def test_build_check_on_compiled_code(tmp_path, wait, ok):
     else:
         with pytest.raises(RuntimeError, match="untracked LDS reads used before their wait"):
             _build._check_untracked_reads(src, verbose=False, out_dir=tmp_path)
+
+
+def test_a_module_that_cannot_be_compiled_does_not_take_the_optimizer_along(monkeypatch):
+    """Both CPython modules: a warning that says what is missing; the library is built without them."""
+    monkeypatch.setattr(_build, "_build_module", lambda *_: "\nno headers")
+    with pytest.warns(RuntimeWarning, match="_layout was not built"):
+        _build._build_layout(False)
+    with pytest.warns(RuntimeWarning, match="_objectives was not built: calling an objective will raise.*\n*no headers"):
+        _build._build_objectives(False)
