@@ -355,7 +355,7 @@ int mamw_token_logprobs(const mamw_rows* logits, const mamw_per_row* tokens,
 /* grad_j = (a [j = token] - q_j (a + h (log q_j + entropy))) / T with
  * a = scale * coef[r], h = scale * entropy_coef[r] (no such term where
  * entropy_coef is NULL) and *scale on the device (NULL: 1).  A row whose a and h
- * are 0 is not read and gets zeros, whatever it holds.                        */
+ * are 0 gets zeros, whatever it holds.                                        */
 int mamw_logits_grad(const mamw_rows* logits, const mamw_per_row* tokens,
                      int64_t ignore_index, float temperature,
                      const float* stats, const mamw_per_row* coef,

@@ -467,7 +467,7 @@ struct HeldRow {
             }
     }
 
-    // The wave's statistics.  hold(vector, i) is applied to held vector i, change(vector, number) to those that are not
+    // The thread's statistics.  hold(vector, i) is applied to held vector i, change(vector, number) to those that are not
     // held.  With kRest those held are loaded last, for the registers.
     template <typename Hold, typename Change>
     __device__ __forceinline__ Stats stats(float c, Hold hold, Change change) {
@@ -510,7 +510,7 @@ struct HeldRow {
                 }
                 __builtin_amdgcn_sched_barrier(0);  // the next group is not begun, and waited for, before
             }
-        return over_wave<false>(st, c);
+        return st;
     }
 
     // g_j = b 2^y below m.

@@ -188,8 +188,8 @@ __device__ __forceinline__ float moved(float p, float from, float to) {
 }
 
 // p (x - top) goes by the entries' own largest logit: a wave may see nothing but the type's lowest value in the row, and
-// a difference to that would have lost x.
-template <int kThreads_>
+// a difference to that would have lost x.  (p is the wave's afterwards, too.)
+template <int kThreads_, bool kTail>
 __device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* lds) {
     constexpr int kN = kThreads_ / 64;
     if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = mine;
@@ -202,13 +202,12 @@ __device__ __forceinline__ Parts parts_over_block(Parts mine, float c, Parts* ld
         top = fmaxf(top, __shfl_xor(top, o, 64));
     }
     mine.s *= factor(mine.m, m, c);
-    mine.s_in *= factor(mine.top, top, c);
+    if (kTail) mine.s_in *= factor(mine.top, top, c);
     mine.px += moved(mine.p, mine.top, top);
 #pragma unroll
     for (int o = kN / 2; o >= 1; o >>= 1) {
         mine.s += __shfl_xor(mine.s, o, 64);
-        mine.s_in += __shfl_xor(mine.s_in, o, 64);
-        mine.p += __shfl_xor(mine.p, o, 64);
+        if (kTail) mine.s_in += __shfl_xor(mine.s_in, o, 64);
         mine.px += __shfl_xor(mine.px, o, 64);
     }
     mine.m = m;
@@ -374,32 +373,45 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
                 if (bits) Mark::leave_out(v, bits);
             }
     };
-    const Stats wave = held.stats(x.c, hold, change);
-    float top = -INFINITY;
+    Stats st = held.stats(x.c, hold, change);
+    // Both maxima over the wave, then all sums, side by side, and no more of the entries' slots than k fills: with
+    // one after the other 65536 x 1003 bf16 took 131 us instead of 130, 134 instead of 133 with a rest.
+    float m_wave = st.m, top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kEntries; ++e)
-        if (index[e] >= 0) top = fmaxf(top, xs[e].value());
-    top = wave_max(top);
+        if (e * kThreads_ < p.k && index[e] >= 0) top = fmaxf(top, xs[e].value());
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        m_wave = fmaxf(m_wave, __shfl_xor(m_wave, o, 64));
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+    }
+    move_to<false>(st, m_wave, x.c);
     const float ref_top = reference(top);
-    float s_in = 0.f, sum_p = 0.f, px_in = 0.f;
+    float s_wave = st.s, s_in = 0.f, sum_p = 0.f, px_in = 0.f;
 #pragma unroll
     for (int e = 0; e < kEntries; ++e) {
-        if (index[e] < 0) continue;
+        if (e * kThreads_ >= p.k || index[e] < 0) continue;
         if (kTail) s_in += __builtin_amdgcn_exp2f(below(xs[e].value(), ref_top, x.c));
         sum_p += probs[e];
         px_in += probs[e] > 0.f ? probs[e] * (xs[e].value() - ref_top) : probs[e];  // 0 * -inf; NaN stays
     }
-    const Parts all_parts = parts_over_block<kThreads_>(
-        {wave.m, wave.s, top, wave_sum(s_in), wave_sum(sum_p), wave_sum(px_in)}, x.c, lds);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        s_wave += __shfl_xor(s_wave, o, 64);
+        if (kTail) s_in += __shfl_xor(s_in, o, 64);
+        sum_p += __shfl_xor(sum_p, o, 64);
+        px_in += __shfl_xor(px_in, o, 64);
+    }
+    const Parts all_parts = parts_over_block<kThreads_, kTail>({m_wave, s_wave, top, s_in, sum_p, px_in}, x.c, lds);
     // m, rest: of what the row holds; all, s: with the teacher's entries
     const float m = all_parts.m, rest = all_parts.s, all = kTail ? fmaxf(m, all_parts.top) : m;
     const float m_to_all = kTail ? factor(m, all, x.c) : 1.f;
     const float s = kTail ? rest * m_to_all + all_parts.s_in * factor(all_parts.top, all, x.c) : rest, inv_s = 1.f / s;
     // sum p (log p - log q), with log q = (x - all) / T - log s
-    const float px = all_parts.px + moved(all_parts.p, all_parts.top, all);
+    const float px = all_parts.px + moved(teacher.sum_p, all_parts.top, all);
     float loss = teacher.entries > 0 ? teacher.plogp - px * x.inv_t + teacher.sum_p * logf(s) : 0.f;
     float in = teacher.entries > 0 ? 1.f : 0.f;  // times inv_s 2^y: A q_j
-    float outside = in * inv_s;                     // times 2^y below m: A q_j - P q_j / Q, outside the entries
+    float outside = in * inv_s;                  // times 2^y below m: A q_j - P q_j / Q, outside the entries
     if constexpr (kTail) {
         in = teacher.sum_p;
         if (teacher.entries < x.vocab) {

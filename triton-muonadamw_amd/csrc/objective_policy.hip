@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void policy_kernel(
     const float ref = p.ref.data ? load_f32(p.ref, at) : 0.f;
     HeldRow<T, kThreads_, kVecs, kRest> held;
     held.load(row, x.vocab, p.count);
-    const Stats wave = held.stats(x.c, Unchanged(), Unchanged());
+    const Stats wave = over_wave<false>(held.stats(x.c, Unchanged(), Unchanged()), x.c);
     const Stats st = over_block<false, kThreads_>(wave, x.c, lds);
     const float w = 1.f / (length * counted.all());
     const float xt = chosen.value();

@@ -94,17 +94,13 @@ __global__ __launch_bounds__(kThreads) void logits_grad_kernel(Rows x, PerRow to
     for (uint32_t back = blockIdx.y; back < uint32_t(x.rows); back += gridDim.y) {
         const uint32_t r = uint32_t(x.rows) - 1 - back;
         const Place at = place(x, r);
-        const float row_coef = load_f32(coef, at), row_entropy_coef = kEntropy ? load_f32(entropy_coef, at) : 0.f;
         const int64_t token = load_int(tokens, offset(tokens, at));
-        const bool beyond = token < 0 || token >= x.vocab;
-        const float a = beyond ? NAN : f * row_coef, h = f * row_entropy_coef;
         T* g = grad + int64_t(r) * x.vocab;
         const T* row = row_of<T>(x, at);
         const Span span = span_of(row, x.vocab);
         const int from = int(part) * kGradVecs, t = threadIdx.x;
         T* to = g + span.head;
-        // Nor does a row count that nothing depends on: outside all pairs, it may hold anything.
-        if (token == ignore || (a == 0.f && h == 0.f)) {
+        auto zeros = [&] {
 #pragma unroll
             for (int u = 0; u < kGradUnroll; ++u) {
                 const int n = from + u * kThreads;
@@ -112,6 +108,9 @@ __global__ __launch_bounds__(kThreads) void logits_grad_kernel(Rows x, PerRow to
             }
             if (part == 0 && int(threadIdx.x) < span.extra)
                 g[extra_element<T>(span, threadIdx.x)] = narrow<T>(0.f);
+        };
+        if (token == ignore) {
+            zeros();
             continue;
         }
         vec_t v[kGradUnroll];
@@ -121,6 +120,16 @@ __global__ __launch_bounds__(kThreads) void logits_grad_kernel(Rows x, PerRow to
             v[u] = n + t < span.vecs ? load_vec(row + span.head, n, t) : nothing<T>();
         }
         const float m = stats[2 * int64_t(r)], s = stats[2 * int64_t(r) + 1], inv_s = 1.f / s;
+        const bool beyond = token < 0 || token >= x.vocab;
+        const float a = beyond ? NAN : f * load_f32(coef, at);
+        const float h = kEntropy ? f * load_f32(entropy_coef, at) : 0.f;
+        // Nor does a row count that nothing depends on: outside all pairs, it may hold anything.  (It is loaded all the same:
+        // with the question in front, every row's loads wait for its coefficient, 306 -> 312 us for 8192 x 50257 bf16 with
+        // entropies and both directions.)
+        if (a == 0.f && h == 0.f) {
+            zeros();
+            continue;
+        }
         // a + h (log q + H) = b + h ln2 y
         const float b = kEntropy ? a + h * (entropy[r] - logf(s)) : a, hy = h * kLn2;
         auto value = [&](float xj, int j) {
