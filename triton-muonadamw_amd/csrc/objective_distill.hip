@@ -280,8 +280,8 @@ struct Marks {
 //
 // One read and one write, as in the policy's kernel: 4096 x 128256 bf16 with 128 entries and a rest, 2409 rows that
 // count, 0.62 GB read and 1.05 written in 325 us, 5.1 TB/s; 2048 x 50257 fp32 with 64 entries, 0.14 and 0.41 GB, in 99,
-// 5.6 TB/s.  Writing the entries over what the row's vectors left is 4 of these 325 us and as many as 20 to 28 of 265
-// where rows are short (65536 x 4000, 64 entries); the gathers of the entries' logits are 14 there.
+// 5.6 TB/s.  Writing the entries over what the row's vectors left is 4 of these 325 us and as many as 20 to 28 of the 222
+// of 65536 x 4000 bf16 with 64 entries, 35592 rows that count; the gathers of the entries' logits are 14 there.
 template <typename T, int kThreads_, int kVecs, bool kRest, bool kTail>
 __global__ __launch_bounds__(kThreads_, kRowWaves<kVecs>) void distill_kernel(
     Rows x, Distill p, Result out, const float* __restrict__ scale, int unless_one,
